@@ -55,7 +55,7 @@ def _torch_paths():
 def _sources():
     kernels = sorted((CSRC / "kernels").glob("*.hip"))
     runtime = sorted((CSRC / "runtime").glob("*.cpp"))
-    return kernels, runtime, CSRC / "bindings.cpp"
+    return kernels, runtime, sorted(CSRC.glob("bindings*.cpp"))
 
 
 def _headers_mtime() -> float:
@@ -73,7 +73,7 @@ def _compile(src: Path, obj: Path, flags: list[str]) -> tuple[Path, str]:
 
 def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
           measure: bool = False) -> Path:
-    kernels, runtime, binding = _sources()
+    kernels, runtime, bindings = _sources()
     obj_dir = OBJ.parent / "obj_measure" if measure else OBJ
     obj_dir.mkdir(parents=True, exist_ok=True)
     flavor = "measure" if measure else "production"
@@ -101,9 +101,10 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
         obj = obj_dir / (src.stem + ".cpp.o")
         objs.append(obj)
         jobs_todo.append((src, obj, base))
-    obj_b = obj_dir / "bindings.o"
-    objs.append(obj_b)
-    jobs_todo.append((binding, obj_b, torch_flags))
+    for src in bindings:
+        obj = obj_dir / (src.stem + ".o")
+        objs.append(obj)
+        jobs_todo.append((src, obj, torch_flags))
 
     stale = [(s, o, f) for (s, o, f) in jobs_todo
              if force or not o.exists() or o.stat().st_mtime < max(s.stat().st_mtime, hdr_t)]

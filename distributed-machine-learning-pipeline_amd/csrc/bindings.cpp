@@ -257,6 +257,8 @@ RcclComm* live(PyComm& s) {
 
 }  // namespace
 
+void bind_experts(py::module_& m);  // bindings_experts.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "hipdsml native MI355X (gfx950) kernels and device runtime";
 
@@ -1284,4 +1286,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     if (hipGetDeviceCount(&n) != hipSuccess) n = 0;
     return n;
   });
+
+  // ---- expert layer, gradient clipping --------------------------------------
+  bind_experts(m);
 }

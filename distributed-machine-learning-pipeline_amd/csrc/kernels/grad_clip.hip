@@ -1,0 +1,253 @@
+// Global norm of many gradient tensors, and clipping by it:
+//
+//   norm = sqrt(sum over tensors and elements of g^2)
+//   out  = g * min(1, max_norm / (norm + eps))       (out may be g itself)
+//
+// Squares are summed in fp64 (any finite fp32 gradient's square is finite
+// there, and the sum loses nothing that matters over 1e9 elements; the kernel
+// waits for bytes, not for arithmetic).  Two passes: the first leaves one fp64
+// partial per workgroup, every workgroup of the second sums all of them in
+// the same order -- no atomics, so the result does not depend on timing -- and
+// scales its share.  Tensors are cut into pieces of 4096 16-B words; a
+// workgroup takes every gridDim-th piece.  The tensor table travels in the
+// kernel arguments, so a call keeps nothing on the device and can be captured.
+#include <algorithm>
+
+#include "common.h"
+#include "../dsml.h"
+#include "../experts.h"
+
+namespace dsml {
+namespace {
+
+constexpr int kGnThreads = 256;
+constexpr int kGnMax = 128;            // tensors of one launch (3.6 KB of arguments)
+constexpr int kGnPiece = 4096;         // 16-B words of one piece
+constexpr int kGnBlocks = 1024;        // workgroups over all launches, about
+
+struct GnTable {
+  const void* g[kGnMax];
+  void* out[kGnMax];
+  int64_t n[kGnMax];
+  uint32_t start[kGnMax + 1];  // first piece of each tensor
+  int count;
+};
+
+template <int DT>
+constexpr int gn_per() { return DT == kF32 ? 4 : 8; }
+
+template <int DT>
+__device__ __forceinline__ float gn_ld(const void* p, int64_t i) {
+  if constexpr (DT == kF32) return static_cast<const float*>(p)[i];
+  else if constexpr (DT == kBF16) return bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
+  else return __half2float(static_cast<const __half*>(p)[i]);
+}
+template <int DT>
+__device__ __forceinline__ void gn_st(void* p, int64_t i, float v) {
+  if constexpr (DT == kF32) static_cast<float*>(p)[i] = v;
+  else if constexpr (DT == kBF16) static_cast<uint16_t*>(p)[i] = f32_to_bf16(v);
+  else static_cast<__half*>(p)[i] = __float2half(v);
+}
+template <int DT>
+__device__ __forceinline__ void gn_unpack(uint4 u, float (&f)[gn_per<DT>()]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < gn_per<DT>(); ++i) {
+    if constexpr (DT == kF32) f[i] = __uint_as_float(w[i]);
+    else if constexpr (DT == kBF16) f[i] = bf16_to_f32((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+    else f[i] = __half2float(__ushort_as_half((uint16_t)(w[i >> 1] >> (16 * (i & 1)))));
+  }
+}
+template <int DT>
+__device__ __forceinline__ uint4 gn_pack(const float (&f)[gn_per<DT>()]) {
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < gn_per<DT>(); ++i) {
+    if constexpr (DT == kF32) w[i] = __float_as_uint(f[i]);
+    else if constexpr (DT == kBF16) w[i >> 1] |= (uint32_t)f32_to_bf16(f[i]) << (16 * (i & 1));
+    else w[i >> 1] |= (uint32_t)__half_as_ushort(__float2half(f[i])) << (16 * (i & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Tensor of piece p (uniform over the workgroup).
+__device__ __forceinline__ int gn_find(const GnTable& t, uint32_t p) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (t.start[mid] <= p) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ double gn_block_sum(double v, double* lds) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+  const int w = threadIdx.x >> 6;
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[w] = v;
+  __syncthreads();
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kGnThreads / 64; ++i) s += lds[i];
+  return s;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kGnThreads) void grad_sq_k(GnTable t, double* part) {
+  __shared__ double lds[kGnThreads / 64];
+  constexpr int P = gn_per<DT>();
+  double acc = 0.0;
+  const uint32_t pieces = t.start[t.count];
+  for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
+    const int i = gn_find(t, p);
+    const void* g = t.g[i];
+    const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * kGnPiece * P;
+    const int64_t last = first + (int64_t)kGnPiece * P < n ? first + (int64_t)kGnPiece * P : n;
+    if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+      const uint4* v = reinterpret_cast<const uint4*>(g);
+      const int64_t v1 = last / P;
+      for (int64_t k = first / P + threadIdx.x; k < v1; k += kGnThreads) {
+        float f[P];
+        gn_unpack<DT>(v[k], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) acc = fma((double)f[j], (double)f[j], acc);
+      }
+      for (int64_t k = v1 * P + threadIdx.x; k < last; k += kGnThreads) {
+        const double x = gn_ld<DT>(g, k);
+        acc = fma(x, x, acc);
+      }
+    } else {
+      for (int64_t k = first + threadIdx.x; k < last; k += kGnThreads) {
+        const double x = gn_ld<DT>(g, k);
+        acc = fma(x, x, acc);
+      }
+    }
+  }
+  const double s = gn_block_sum(acc, lds);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+__device__ __forceinline__ double gn_total(const double* part, int parts, double* lds) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < parts; i += kGnThreads) s += part[i];
+  return gn_block_sum(s, lds);
+}
+
+__global__ __launch_bounds__(kGnThreads) void grad_norm_k(const double* part, int parts, float* norm) {
+  __shared__ double lds[kGnThreads / 64];
+  const double s = gn_total(part, parts, lds);
+  if (threadIdx.x == 0) norm[0] = (float)sqrt(s);
+}
+
+// Every workgroup sums the partials in the same order, so all scale by the same value.
+template <int DT>
+__global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const double* part, int parts, float* norm,
+                                                           double max_norm, double eps) {
+  __shared__ double lds[kGnThreads / 64];
+  constexpr int P = gn_per<DT>();
+  const double nrm = sqrt(gn_total(part, parts, lds));
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)nrm;
+  double cd = max_norm / (nrm + eps);
+  cd = cd > 1.0 ? 1.0 : cd;  // NaN stays NaN: a broken gradient is not hidden
+  const float c = (float)cd;
+  const uint32_t pieces = t.start[t.count];
+  for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
+    const int i = gn_find(t, p);
+    const void* g = t.g[i];
+    void* o = t.out[i];
+    if (c == 1.f && o == g) continue;  // nothing changes
+    const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * kGnPiece * P;
+    const int64_t last = first + (int64_t)kGnPiece * P < n ? first + (int64_t)kGnPiece * P : n;
+    if (((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
+      const uint4* v = reinterpret_cast<const uint4*>(g);
+      uint4* w = reinterpret_cast<uint4*>(o);
+      const int64_t v1 = last / P;
+      for (int64_t k = first / P + threadIdx.x; k < v1; k += kGnThreads) {
+        float f[P];
+        gn_unpack<DT>(v[k], f);
+#pragma unroll
+        for (int j = 0; j < P; ++j) f[j] *= c;
+        w[k] = gn_pack<DT>(f);
+      }
+      for (int64_t k = v1 * P + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, gn_ld<DT>(g, k) * c);
+    } else {
+      for (int64_t k = first + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, gn_ld<DT>(g, k) * c);
+    }
+  }
+}
+
+int64_t gn_pieces(int64_t n, int P) {
+  const int64_t per = (int64_t)kGnPiece * P;
+  return (n + per - 1) / per;
+}
+// Workgroups of one launch: its share of the pieces of the whole call.
+int gn_grid(int64_t pieces, int64_t all) {
+  if (pieces <= 0) return 1;
+  int64_t g = all <= kGnBlocks ? pieces : (pieces * kGnBlocks + all - 1) / all;
+  return (int)std::max<int64_t>(1, g);
+}
+
+}  // namespace
+
+int64_t grad_norm_ws_doubles(const int64_t* n, int count) {
+  // every launch rounds its share up by at most one workgroup
+  (void)n;
+  return kGnBlocks + (count + kGnMax - 1) / kGnMax + 1;
+}
+
+template <int DT>
+static hipError_t run_norm(const ClipTensor* t, int count, double* ws, float* norm, bool clip, double max_norm,
+                           double eps, hipStream_t s) {
+  constexpr int P = gn_per<DT>();
+  int64_t all = 0;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].n < 0 || gn_pieces(t[i].n, P) > 0x3fffffffLL) return hipErrorInvalidValue;
+    all += gn_pieces(t[i].n, P);
+  }
+  int parts = 0;
+  for (int pass = 0; pass < (clip ? 2 : 1); ++pass) {
+    for (int i0 = 0; i0 < count; i0 += kGnMax) {
+      GnTable tb;
+      tb.count = std::min(kGnMax, count - i0);
+      int64_t pieces = 0;
+      for (int i = 0; i < tb.count; ++i) {
+        tb.g[i] = t[i0 + i].g;
+        tb.out[i] = t[i0 + i].out;
+        tb.n[i] = t[i0 + i].n;
+        tb.start[i] = (uint32_t)pieces;
+        pieces += gn_pieces(t[i0 + i].n, P);
+        if (pieces > 0x7fffffffLL) return hipErrorInvalidValue;
+      }
+      tb.start[tb.count] = (uint32_t)pieces;
+      const int grid = gn_grid(pieces, all);
+      if (pass == 0) {
+        hipLaunchKernelGGL((grad_sq_k<DT>), dim3(grid), dim3(kGnThreads), 0, s, tb, ws + parts);
+        parts += grid;
+      } else {
+        hipLaunchKernelGGL((grad_scale_k<DT>), dim3(grid), dim3(kGnThreads), 0, s, tb, ws, parts,
+                           i0 == 0 ? norm : nullptr, max_norm, eps);
+      }
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+  }
+  if (!clip || count == 0) {
+    hipLaunchKernelGGL(grad_norm_k, dim3(1), dim3(kGnThreads), 0, s, ws, parts, norm);
+    return hipGetLastError();
+  }
+  return hipSuccess;
+}
+
+hipError_t grad_norm(const ClipTensor* t, int count, int dtype, double* ws, float* norm, bool clip, double max_norm,
+                     double eps, hipStream_t s) {
+  switch (dtype) {
+    case kF32: return run_norm<kF32>(t, count, ws, norm, clip, max_norm, eps, s);
+    case kBF16: return run_norm<kBF16>(t, count, ws, norm, clip, max_norm, eps, s);
+    case kF16: return run_norm<kF16>(t, count, ws, norm, clip, max_norm, eps, s);
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace dsml

@@ -4,6 +4,8 @@ the simulated device runtime).
 """
 from __future__ import annotations
 
+from typing import List, Optional, Sequence
+
 import torch
 
 from .native import require_native
@@ -92,3 +94,57 @@ def scale_(x: torch.Tensor, alpha: float) -> torch.Tensor:
     else:
         x.mul_(alpha)
     return x
+
+
+def _norm_ref(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    return sum(g.double().square().sum() for g in grads).sqrt()
+
+
+def _check_grads(grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]]) -> None:
+    if not grads:
+        raise RuntimeError("no gradients given")
+    if grads[0].dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise RuntimeError("gradients must be float32, bfloat16 or float16")
+    if any(g.dtype != grads[0].dtype for g in grads):
+        raise RuntimeError("gradients must have one type")
+    if any(not g.is_contiguous() for g in grads):
+        raise RuntimeError("gradients must be contiguous")
+    if out is not None:
+        if len(out) != len(grads):
+            raise RuntimeError("out must hold one tensor a gradient")
+        if any(o.dtype != g.dtype for o, g in zip(out, grads)):
+            raise RuntimeError("out must have the gradients' type")
+        if any(not o.is_contiguous() or o.shape != g.shape for o, g in zip(out, grads)):
+            raise RuntimeError("out must be contiguous and of the gradients' shapes")
+    if any(t.is_cuda for t in list(grads) + list(out or [])):
+        raise RuntimeError("gradients must be on one device")
+
+
+def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
+    """``sqrt(sum g^2)`` over every element of every gradient (float32, bfloat16
+    or float16, one type, contiguous), as a 0-dim float32 tensor on their device:
+    nothing is copied to the host.  Squares are summed in float64."""
+    grads = list(grads)
+    if grads and grads[0].is_cuda:
+        return require_native().grad_norm(grads)
+    _check_grads(grads, None)
+    return _norm_ref(grads).float()
+
+
+def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float = 1e-6,
+                    out: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
+    """Scale the gradients by ``min(1, max_norm / (norm + eps))`` and return their
+    norm before that.  In place, or into the tensors of ``out`` (the gradients
+    then stay as they are).  A norm that is not a number makes every gradient so
+    too; an infinite one makes them 0 (not a number where they are infinite)."""
+    grads = list(grads)
+    if grads and grads[0].is_cuda:
+        return require_native().grad_norm(grads, True, float(max_norm), float(eps), out)
+    if not max_norm >= 0:
+        raise RuntimeError(f"max_norm must not be negative, got {max_norm}")
+    _check_grads(grads, out)
+    norm = _norm_ref(grads)
+    coef = torch.clamp(max_norm / (norm + eps), max=1.0).float()
+    for g, o in zip(grads, grads if out is None else out):
+        o.copy_(g.float() * coef)
+    return norm.float()
