@@ -81,7 +81,10 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
     relink = not stamp.exists() or stamp.read_text().strip() != flavor
     inc, lib, abi = _torch_paths()
     extra = ["-DHIPDSML_MEASURE"] if measure else []
+    # no packed fp32 instructions: the compiler forms v_pk_{add,mul,fma}_f32 from
+    # ordinary float code, and some of their forms are not reliable on this hardware
     base = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I", str(CSRC),
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
             "-Wno-unused-result", "-Wno-pass-failed"] + extra
     host_only = ["-O3", "-std=c++17", "-fPIC", "-I", str(CSRC), "-D__HIP_PLATFORM_AMD__=1",
                  "-Wno-unused-result"] + extra
