@@ -225,6 +225,363 @@ hipError_t launch_any(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// Fast path: widths and row strides of whole 16-B words.  256 x 256 output
+// tile, 64-deep steps, 8 waves of 128 x 64 (16x16x32 MFMA), operands by LDS-DMA
+// into two buffers.
+// ---------------------------------------------------------------------------
+typedef __attribute__((address_space(3))) void* gg_lptr;
+typedef short gg_i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) gg_i16x4* gg_lv4;
+typedef uint32_t gg_u4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kGgOob = 0xfffffff0u;    // past every buffer: reads 0
+constexpr int64_t kGgSpan = 0xffffff00LL;   // bytes a buffer descriptor may span
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t gg_rsrc(const void* base, int64_t bytes) {
+  const uint32_t n = bytes <= 0 ? 0u : (bytes > kGgSpan ? (uint32_t)kGgSpan : (uint32_t)bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, n, 0x00020000);
+}
+// A value every lane holds, in scalar registers.
+__device__ __forceinline__ int64_t gg_uni(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)v >> 32));
+  return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ const char* gg_uni(const char* v) { return reinterpret_cast<const char*>(gg_uni((int64_t)v)); }
+template <int IMM>
+__device__ __forceinline__ void gg_dma(__amdgpu_buffer_rsrc_t r, char* lds, uint32_t vo, uint32_t so) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (gg_lptr)lds, 16, vo, so, IMM, 0);
+}
+// 16-B chunk swizzles of a 128-B LDS row: row-major operands (rows of 64
+// reduction elements) and transposed ones (64 reduction rows of 64 columns).
+__device__ __forceinline__ int gg_swz(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int gg_swz_tr(int r) { return 2 * (((r >> 1) & 1) | (((r >> 3) & 1) << 1)); }
+
+// One operand of the product as a stream of 64-deep steps into LDS images.
+// TR false: R rows of 128 B; TR true: R / 64 images of [64][128 B].
+template <int R, int WAVES, bool TR>
+struct GgOperand {
+  static constexpr int kPieces = R / 8 / WAVES;  // 1-KiB pieces of a step, a wave
+  const char* base;
+  int64_t bytes;   // behind base, all rows
+  int64_t step;    // bytes the base moves a step (TR)
+  uint32_t vo[kPieces];
+  int c8;          // !TR: this lane's first element in a step
+
+  __device__ __forceinline__ void issue(char* lds, int t, int w, int left) {
+    if constexpr (!TR) {
+      const __amdgpu_buffer_rsrc_t r = gg_rsrc(base, bytes);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j)  // a reduction tail reads 0
+        gg_dma<0>(r, lds + (w + WAVES * j) * 1024, c8 < left ? vo[j] : kGgOob, (uint32_t)t * 128u);
+    } else {
+      const __amdgpu_buffer_rsrc_t r = gg_rsrc(base + t * step, bytes - t * step);
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) {
+        const int piece = w + WAVES * j;  // row group piece & 7 of image piece >> 3
+        gg_dma<0>(r, lds + ((piece >> 3) * 8 + (piece & 7)) * 1024, vo[j], 0);
+      }
+    }
+  }
+};
+
+template <int DT, bool TR, int NF>
+struct GgFrags {
+  gg_u4 v[NF];
+  // fragments of 16 rows (columns when TR) each, from wbase on; h: half of the 64-deep step
+  __device__ __forceinline__ void load(const char* lds, int wbase, int h, int lane) {
+    if constexpr (!TR) {
+      const int i = lane & 15, g = lane >> 4;
+      const char* p = lds + (wbase + i) * 128 + 16 * ((4 * h + g) ^ gg_swz(i));
+#pragma unroll
+      for (int x = 0; x < NF; ++x) v[x] = *reinterpret_cast<const gg_u4*>(p + x * 2048);
+    } else {
+      const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
+      const int r0 = 32 * h + 8 * g + q;
+#pragma unroll
+      for (int x = 0; x < NF; ++x) {
+        const int col = wbase + 16 * x;
+        const char* img = lds + (col >> 6) * 8192;
+        const int chunk = ((col & 63) >> 3) + (pp >> 1);
+        const char* a = img + r0 * 128 + 16 * (chunk ^ gg_swz_tr(r0)) + 8 * (pp & 1);
+        const gg_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(a));
+        const gg_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(a + 512));
+        const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+        v[x] = gg_u4{l2.x, l2.y, h2.x, h2.y};
+      }
+    }
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ f32x4 gg_mfma(gg_u4 a, gg_u4 b, f32x4 c) {
+  return gg_mfma16<DT>(__builtin_bit_cast(uint4, a), __builtin_bit_cast(uint4, b), c);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t gg_pack2(float a, float b) {  // round to nearest even
+  if constexpr (DT == kBF16) {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, v2{(__bf16)a, (__bf16)b});
+  } else {
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, v2{(_Float16)a, (_Float16)b});
+  }
+}
+
+// BM x BN tile, WM x WN waves.
+template <int DT, int OP, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a, int mt_max, int nt) {
+  constexpr int W = WM * WN, XF = BM / WM / 16, YF = BN / WN / 16;
+  constexpr bool TA = OP == kWgrad, TB = OP != kLinear;
+  __shared__ __attribute__((aligned(1024))) char a0[BM * 128], b0[BN * 128], a1[BM * 128], b1[BN * 128];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rr = lane >> 3, p = lane & 7;
+  const char* A = static_cast<const char*>(a.a);
+  const char* B = static_cast<const char*>(a.b);
+  const int cols = OP == kLinear ? a.N : a.K;
+
+  // ---- which tile ----
+  int e, mrows;           // expert (-1: rows to zero), rows of this tile
+  int64_t m0, red0 = 0;   // first output row; first reduction row (wgrad)
+  int red;                // reduction length
+  int n0;
+  if constexpr (OP == kWgrad) {
+    const int per = mt_max * nt;
+    const int e_ = blockIdx.x / per, r = blockIdx.x % per;
+    e = e_;
+    m0 = (int64_t)(r / nt) * BM;
+    n0 = (r % nt) * BN;
+    mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
+    red0 = gg_clamp(a.offsets[e], 0, a.S);
+    red = (int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0);
+  } else {
+    const int mt = blockIdx.x / nt;
+    n0 = (blockIdx.x % nt) * BN;
+    const GgTile t = gg_find(a.offsets, a.E, a.S, BM, mt, a.zero_rest);
+    if (t.e == -2) return;
+    e = __builtin_amdgcn_readfirstlane(t.e);
+    m0 = __builtin_amdgcn_readfirstlane((int)t.s0);
+    mrows = __builtin_amdgcn_readfirstlane((int)(t.s1 - t.s0));
+    red = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
+  }
+  const int ncols = cols - n0 < BN ? cols - n0 : BN;
+
+  // ---- operand streams ----
+  GgOperand<BM, W, TA> oa;
+  GgOperand<BN, W, TB> ob;
+  if constexpr (!TA) {
+    oa.c8 = 8 * (p ^ gg_swz(8 * w + rr));
+    const bool gather = OP == kLinear && a.rows;
+    oa.base = gather ? A : A + m0 * a.lda * 2;
+    oa.bytes = gather ? ((a.T - 1) * a.lda + a.K) * 2 : ((int64_t)(mrows - 1) * a.lda + red) * 2;
+#pragma unroll
+    for (int j = 0; j < oa.kPieces; ++j) {
+      const int r = 8 * (w + W * j) + rr;
+      int64_t row = r;
+      bool ok = r < mrows;
+      if (gather) {
+        row = ok && e >= 0 ? a.rows[m0 + r] : 0;
+        ok = ok && row >= 0 && row < a.T;
+      }
+      oa.vo[j] = ok ? (uint32_t)((row * a.lda + oa.c8) * 2) : kGgOob;
+    }
+  } else {
+    const int r = 8 * (w & 7) + rr;
+    oa.base = A + (red0 * a.lda + m0) * 2;
+    oa.bytes = ((int64_t)(red - 1) * a.lda + mrows) * 2;
+    oa.step = 64 * a.lda * 2;
+#pragma unroll
+    for (int j = 0; j < oa.kPieces; ++j) {
+      const int c = 64 * ((w + W * j) >> 3) + 8 * (p ^ gg_swz_tr(r));
+      oa.vo[j] = c < mrows ? (uint32_t)((r * a.lda + c) * 2) : kGgOob;
+    }
+  }
+  if constexpr (!TB) {
+    ob.c8 = 8 * (p ^ gg_swz(8 * w + rr));
+    ob.base = B + ((int64_t)e * a.strb + (int64_t)n0 * a.ldb) * 2;
+    ob.bytes = ((int64_t)(ncols - 1) * a.ldb + red) * 2;
+#pragma unroll
+    for (int j = 0; j < ob.kPieces; ++j) {
+      const int r = 8 * (w + W * j) + rr;
+      ob.vo[j] = r < ncols ? (uint32_t)((r * a.ldb + ob.c8) * 2) : kGgOob;
+    }
+  } else {
+    const int r = 8 * (w & 7) + rr;
+    ob.base = OP == kDgrad ? B + ((int64_t)e * a.strb + n0) * 2 : B + (red0 * a.ldb + n0) * 2;
+    ob.bytes = ((int64_t)(red - 1) * a.ldb + ncols) * 2;
+    ob.step = 64 * a.ldb * 2;
+#pragma unroll
+    for (int j = 0; j < ob.kPieces; ++j) {
+      const int c = 64 * ((w + W * j) >> 3) + 8 * (p ^ gg_swz_tr(r));
+      ob.vo[j] = c < ncols ? (uint32_t)((r * a.ldb + c) * 2) : kGgOob;
+    }
+  }
+
+  oa.base = gg_uni(oa.base);
+  oa.bytes = gg_uni(oa.bytes);
+  ob.base = gg_uni(ob.base);
+  ob.bytes = gg_uni(ob.bytes);
+  red = __builtin_amdgcn_readfirstlane(red);
+  f32x4 acc[XF][YF];
+#pragma unroll
+  for (int x = 0; x < XF; ++x)
+#pragma unroll
+    for (int y = 0; y < YF; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
+  const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
+
+  const int steps = (red + 63) / 64;
+  auto compute = [&](const char* la, const char* lb) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      GgFrags<DT, TA, XF> fa;
+      GgFrags<DT, TB, YF> fb;
+      fa.load(la, wm, h, lane);
+      fb.load(lb, wn, h, lane);
+#pragma unroll
+      for (int x = 0; x < XF; ++x)
+#pragma unroll
+        for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(fb.v[y], fa.v[x], acc[x][y]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto arrived = [&]() {  // this wave's pieces are in LDS, then everybody's
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto stage = [&](char* la, char* lb, int t) {
+    if (t < steps) {
+      oa.issue(la, t, w, red - 64 * t);
+      ob.issue(lb, t, w, red - 64 * t);
+    }
+  };
+  stage(a0, b0, 0);
+  arrived();
+  for (int t = 0; t < steps; t += 2) {
+    stage(a1, b1, t + 1);
+    compute(a0, b0);
+    arrived();
+    stage(a0, b0, t + 2);
+    if (t + 1 < steps) compute(a1, b1);
+    arrived();
+  }
+
+  // ---- epilogue: lane (i, g) holds columns 4 g .. 4 g + 3 of row i of every 16 x 16 tile ----
+  const int i = lane & 15, g = lane >> 4;
+  if constexpr (OP == kWgrad) {
+    float* out = static_cast<float*>(a.out) + (int64_t)e * a.stro;
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      const int m = wm + 16 * x + i;
+      if (m >= mrows) continue;
+      float* o = out + (m0 + m) * a.ldo + n0;
+#pragma unroll
+      for (int y = 0; y < YF; ++y) {
+        const int n = wn + 16 * y + 4 * g;
+        if (n < ncols) *reinterpret_cast<f32x4*>(o + n) = acc[x][y];
+      }
+    }
+  } else {
+    if constexpr (OP == kLinear) {
+      if (e >= 0 && a.bias) {
+#pragma unroll
+        for (int y = 0; y < YF; ++y) {
+          const int n = wn + 16 * y + 4 * g;
+          f32x4 b = {0.f, 0.f, 0.f, 0.f};
+          if (n < ncols) {
+            const float* bp = a.bias + (int64_t)e * a.ldbias + n0 + n;
+            b = f32x4{bp[0], bp[1], bp[2], bp[3]};
+          }
+#pragma unroll
+          for (int x = 0; x < XF; ++x) acc[x][y] += b;
+        }
+      }
+      if (a.relu) {
+#pragma unroll
+        for (int x = 0; x < XF; ++x)
+#pragma unroll
+          for (int y = 0; y < YF; ++y)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[x][y][q] = acc[x][y][q] < 0.f ? 0.f : acc[x][y][q];
+      }
+    }
+    uint16_t* out = static_cast<uint16_t*>(a.out);
+    const uint16_t* mk = OP == kDgrad && e >= 0 ? static_cast<const uint16_t*>(a.mask) : nullptr;
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      const int m = wm + 16 * x + i;
+#pragma unroll
+      for (int y = 0; y < YF; y += 2) {
+        // two neighbouring tiles: lanes of even g take the first, of odd g the
+        // second, 8 columns each
+        uint32_t u0 = gg_pack2<DT>(acc[x][y][0], acc[x][y][1]), u1 = gg_pack2<DT>(acc[x][y][2], acc[x][y][3]);
+        uint32_t v0 = gg_pack2<DT>(acc[x][y + 1][0], acc[x][y + 1][1]);
+        uint32_t v1 = gg_pack2<DT>(acc[x][y + 1][2], acc[x][y + 1][3]);
+        const auto s0 = __builtin_amdgcn_permlane16_swap(u0, v0, false, false);
+        const auto s1 = __builtin_amdgcn_permlane16_swap(u1, v1, false, false);
+        gg_u4 o = {s0[0], s1[0], s0[1], s1[1]};
+        const int n = wn + 16 * (y + (g & 1)) + 8 * (g >> 1);
+        if (m < mrows && n < ncols) {
+          if (mk) {
+            const gg_u4 k = *reinterpret_cast<const gg_u4*>(mk + (m0 + m) * a.ldmask + n0 + n);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const uint32_t lo = gg_f<DT>((uint16_t)k[q]) > 0.f ? 0x0000ffffu : 0u;
+              const uint32_t hi = gg_f<DT>((uint16_t)(k[q] >> 16)) > 0.f ? 0xffff0000u : 0u;
+              o[q] &= lo | hi;
+            }
+          }
+          *reinterpret_cast<gg_u4*>(out + (m0 + m) * a.ldo + n0 + n) = o;
+        }
+      }
+    }
+  }
+}
+
+bool gg_al(const void* p, int64_t ld, int64_t need) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld >= need;
+}
+// Whole 16-B words everywhere, rows that do not overlap, and offsets of 32 bits
+// from each stream's base.
+bool fast_ok(GroupedOp op, const GroupedArgs& a) {
+  if (a.K % 8 || a.N % 8) return false;
+  if (!gg_al(a.a, a.lda, op == kLinear ? a.K : a.N) || !gg_al(a.b, a.ldb, a.K)) return false;
+  if (op != kWgrad && a.E > 1 && a.strb % 8) return false;
+  if (a.lda > 0x7fffff || a.ldb > 0x7fffff) return false;
+  if (op == kLinear && a.rows && (a.T * a.lda + a.K) * 2 > kGgSpan) return false;
+  if (op == kWgrad) return a.rows == nullptr && a.db == nullptr && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0 && (a.E <= 1 || a.stro % 4 == 0);
+  if (!gg_al(a.out, a.ldo, 0)) return false;
+  return op != kDgrad || !a.mask || gg_al(a.mask, a.ldmask, 0);
+}
+
+template <int DT, int OP, int BM, int BN, int WM, int WN>
+hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
+  const int cols = OP == kLinear ? a.N : a.K;
+  const int nt = (cols + BN - 1) / BN;
+  int64_t mt;
+  if (OP == kWgrad) mt = (a.N + BM - 1) / BM;
+  else {
+    mt = (a.S + BM - 1) / BM + a.E + (a.zero_rest ? 2 : 0);
+    mt = mt < a.S ? mt : a.S;
+  }
+  const int64_t blocks = OP == kWgrad ? mt * nt * a.E : mt * nt;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((grouped_fast_k<DT, OP, BM, BN, WM, WN>), dim3((uint32_t)blocks), dim3(64 * WM * WN), 0, s, a,
+                     (int)mt, nt);
+  return hipGetLastError();
+}
+template <int DT>
+hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
+  switch (op) {
+    case kLinear: return launch_fast<DT, kLinear, 256, 256, 2, 4>(a, s);
+    case kDgrad: return launch_fast<DT, kDgrad, 256, 256, 2, 4>(a, s);
+    default: return launch_fast<DT, kWgrad, 256, 256, 2, 4>(a, s);
+  }
+}
+
 }  // namespace
 
 int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a) {
@@ -237,6 +594,7 @@ hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
       (a.dtype != kBF16 && a.dtype != kF16))
     return hipErrorInvalidValue;
   if (op != kWgrad && a.S == 0) return hipSuccess;
+  if (fast_ok(op, a)) return a.dtype == kBF16 ? launch_fast_op<kBF16>(op, a, s) : launch_fast_op<kF16>(op, a, s);
   return a.dtype == kBF16 ? launch_any<kBF16>(op, a, s) : launch_any<kF16>(op, a, s);
 }
 
