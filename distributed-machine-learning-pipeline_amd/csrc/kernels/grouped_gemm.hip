@@ -47,51 +47,67 @@ struct GgTile {
 
 __device__ __forceinline__ int64_t gg_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-// Row tile `mt` in the order: the experts' tiles, then (zero_rest) the tiles of
-// the rows before the first group and behind the last.  One wave scan per 64
-// experts; every wave does it for itself (no LDS, no barrier).
-__device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, int BM, int64_t mt, bool zero_rest) {
+// The groups' row tiles, experts first, then (zero_rest) the tiles of the rows
+// before the first group and behind the last.  `pick` maps the number of tiles
+// to the one wanted (< 0 or too large: nothing).  One wave scan per 64 experts,
+// done by every wave for itself: no LDS, no barrier.
+template <class Pick>
+__device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, int BM, bool zero_rest, Pick pick) {
   const int lane = threadIdx.x & 63;
-  int64_t base = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
+  int a = 0, b = 0, n = 0, inc = 0, tot = 0;
+  auto scan = [&](int e0) {
     const int e = e0 + lane;
-    int64_t a = 0, b = 0;
+    a = b = 0;
     if (e < E) {
-      a = gg_clamp(off[e], 0, S);
-      b = gg_clamp(off[e + 1], a, S);
+      a = (int)gg_clamp(off[e], 0, S);
+      b = (int)gg_clamp(off[e + 1], a, S);
     }
-    const int n = (int)((b - a + BM - 1) / BM);
-    int inc = n;
+    n = (int)(((int64_t)b - a + BM - 1) / BM);
+    inc = n;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
       const int u = __shfl_up(inc, o);
       if (lane >= o) inc += u;
     }
-    const int tot = __shfl(inc, 63);
-    if (mt < base + tot) {
-      const uint64_t hit = __ballot(base + inc > mt);
-      const int l = __ffsll((unsigned long long)hit) - 1;
-      const int64_t first = base + __shfl(inc, l) - __shfl(n, l);
-      const int64_t a0 = __shfl((int)a, l), b0 = __shfl((int)b, l);
-      GgTile t;
-      t.e = e0 + l;
-      t.s0 = a0 + (mt - first) * BM;
-      t.s1 = t.s0 + BM < b0 ? t.s0 + BM : b0;
-      return t;
-    }
-    base += tot;
+    tot = __builtin_amdgcn_readlane(inc, 63);
+  };
+  int total = 0;
+  for (int e0 = (E - 1) & ~63; e0 >= 0; e0 -= 64) {  // the first 64 stay in registers
+    scan(e0);
+    total += tot;
+  }
+  int64_t head = 0, tail = 0;
+  int hn = 0, tn = 0;
+  if (zero_rest) {
+    head = gg_clamp(off[0], 0, S);
+    tail = gg_clamp(off[E], head, S);
+    hn = (int)((head + BM - 1) / BM);
+    tn = (int)((S - tail + BM - 1) / BM);
   }
   GgTile t{-2, 0, 0};
-  if (!zero_rest) return t;
-  const int64_t head = gg_clamp(off[0], 0, S), tail = gg_clamp(off[E], head, S);
-  int64_t r = mt - base;
-  const int64_t hn = (head + BM - 1) / BM;
-  if (r < hn) {
-    t.e = -1; t.s0 = r * BM; t.s1 = t.s0 + BM < head ? t.s0 + BM : head;
-  } else {
-    r -= hn;
-    const int64_t s = tail + r * BM;
-    if (s < S) { t.e = -1; t.s0 = s; t.s1 = s + BM < S ? s + BM : S; }
+  int mt = pick(total + hn + tn);
+  if (mt < 0) return t;
+  if (mt < total) {
+    int e0 = 0;
+    while (mt >= tot) {
+      mt -= tot;
+      e0 += 64;
+      if (e0 >= E) return t;
+      scan(e0);
+    }
+    const int l = __ffsll((unsigned long long)__ballot(inc > mt)) - 1;
+    const int first = __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(n, l);
+    const int64_t a0 = __builtin_amdgcn_readlane(a, l), b0 = __builtin_amdgcn_readlane(b, l);
+    t.e = e0 + l;
+    t.s0 = a0 + (int64_t)(mt - first) * BM;
+    t.s1 = t.s0 + BM < b0 ? t.s0 + BM : b0;
+    return t;
+  }
+  mt -= total;
+  if (mt < hn) {
+    t.e = -1; t.s0 = (int64_t)mt * BM; t.s1 = t.s0 + BM < head ? t.s0 + BM : head;
+  } else if (mt - hn < tn) {
+    t.e = -1; t.s0 = tail + (int64_t)(mt - hn) * BM; t.s1 = t.s0 + BM < S ? t.s0 + BM : S;
   }
   return t;
 }
@@ -119,7 +135,7 @@ __global__ __launch_bounds__(256) void grouped_any_k(GroupedArgs a) {
     r0 = gg_clamp(a.offsets[e], 0, a.S);
     r1 = gg_clamp(a.offsets[e + 1], r0, a.S);
   } else {
-    const GgTile t = gg_find(a.offsets, a.E, a.S, 64, blockIdx.x, a.zero_rest);
+    const GgTile t = gg_find(a.offsets, a.E, a.S, 64, a.zero_rest, [](int) { return (int)blockIdx.x; });
     if (t.e == -2) return;
     e = t.e; m0 = t.s0; m1 = t.s1;
     r0 = 0;
@@ -330,6 +346,16 @@ __device__ __forceinline__ uint32_t gg_pack2(float a, float b) {  // round to ne
   }
 }
 
+// Tile `pos` of an mt x nt grid, in strips of 4 row tiles: neighbours in this
+// order share operands, so a part of it that runs at once on one XCD (32
+// workgroups: 4 x 8 tiles) reads each of them into its L2 once.
+__device__ __forceinline__ void gg_order(int pos, int mt, int nt, int& mi, int& ni) {
+  const int strip = pos / (4 * nt), r = pos - strip * 4 * nt;
+  const int h = mt - 4 * strip < 4 ? mt - 4 * strip : 4;
+  ni = r / h;
+  mi = 4 * strip + (r - ni * h);
+}
+
 // BM x BN tile, WM x WN waves.
 template <int DT, int OP, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a, int mt_max, int nt) {
@@ -348,19 +374,30 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
   int red;                // reduction length
   int n0;
   if constexpr (OP == kWgrad) {
-    const int per = mt_max * nt;
-    const int e_ = blockIdx.x / per, r = blockIdx.x % per;
-    e = e_;
-    m0 = (int64_t)(r / nt) * BM;
-    n0 = (r % nt) * BN;
+    // an expert's tiles, each XCD a contiguous part of them
+    const int per = mt_max * nt, chunk = (per + 7) / 8;
+    const int r = blockIdx.x % (8 * chunk), pos = (r & 7) * chunk + (r >> 3);
+    if (pos >= per) return;
+    e = blockIdx.x / (8 * chunk);
+    int mi, ni;
+    gg_order(pos, mt_max, nt, mi, ni);
+    m0 = (int64_t)mi * BM;
+    n0 = ni * BN;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
     red0 = gg_clamp(a.offsets[e], 0, a.S);
     red = (int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0);
   } else {
-    const int mt = blockIdx.x / nt;
-    n0 = (blockIdx.x % nt) * BN;
-    const GgTile t = gg_find(a.offsets, a.E, a.S, BM, mt, a.zero_rest);
+    int ni = 0;
+    const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
+      const int64_t all = (int64_t)mts * nt, chunk = (all + 7) / 8;
+      const int64_t pos = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
+      if ((blockIdx.x >> 3) >= chunk || pos >= all) return -1;
+      int mi;
+      gg_order((int)pos, mts, nt, mi, ni);
+      return mi;
+    });
     if (t.e == -2) return;
+    n0 = ni * BN;
     e = __builtin_amdgcn_readfirstlane(t.e);
     m0 = __builtin_amdgcn_readfirstlane((int)t.s0);
     mrows = __builtin_amdgcn_readfirstlane((int)(t.s1 - t.s0));
@@ -431,26 +468,32 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
     for (int y = 0; y < YF; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
   const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
 
+  // Fragments of the step's two halves are kept apart, so a half's MFMAs run
+  // while the next half's LDS reads are in flight.  One barrier a step, between
+  // the halves: every wave has then read all of this step (its buffer may be
+  // filled with step t + 2) and step t + 1 has arrived.
   const int steps = (red + 63) / 64;
-  auto compute = [&](const char* la, const char* lb) {
+  GgFrags<DT, TA, XF> fa0, fa1;
+  GgFrags<DT, TB, YF> fb0, fb1;
+  auto mma = [&](const GgFrags<DT, TA, XF>& fa, const GgFrags<DT, TB, YF>& fb) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      GgFrags<DT, TA, XF> fa;
-      GgFrags<DT, TB, YF> fb;
-      fa.load(la, wm, h, lane);
-      fb.load(lb, wn, h, lane);
+    for (int x = 0; x < XF; ++x)
 #pragma unroll
-      for (int x = 0; x < XF; ++x)
+      for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(fb.v[y], fa.v[x], acc[x][y]);
+    // one LDS read, then the MFMAs that hide it
+    constexpr int kReads = XF * (TA ? 2 : 1) + YF * (TB ? 2 : 1), kEach = XF * YF / kReads > 0 ? XF * YF / kReads : 1;
 #pragma unroll
-        for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(fb.v[y], fa.v[x], acc[x][y]);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int q = 0; q < kReads; ++q) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
     }
   };
-  auto arrived = [&]() {  // this wave's pieces are in LDS, then everybody's
-    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  auto arrived = [&]() {  // this wave's pieces are in LDS and its reads done, then everybody's
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
   };
   auto stage = [&](char* la, char* lb, int t) {
     if (t < steps) {
@@ -458,15 +501,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
       ob.issue(lb, t, w, red - 64 * t);
     }
   };
-  stage(a0, b0, 0);
-  arrived();
-  for (int t = 0; t < steps; t += 2) {
-    stage(a1, b1, t + 1);
-    compute(a0, b0);
+  auto step = [&](char* ca, char* cb, const char* na, const char* nb, int t) {
+    fa1.load(ca, wm, 1, lane);
+    fb1.load(cb, wn, 1, lane);
+    mma(fa0, fb0);
     arrived();
-    stage(a0, b0, t + 2);
-    if (t + 1 < steps) compute(a1, b1);
+    stage(ca, cb, t + 2);
+    fa0.load(na, wm, 0, lane);
+    fb0.load(nb, wn, 0, lane);
+    mma(fa1, fb1);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (steps > 0) {
+    stage(a0, b0, 0);
     arrived();
+    stage(a1, b1, 1);
+    fa0.load(a0, wm, 0, lane);
+    fb0.load(b0, wn, 0, lane);
+    for (int t = 0; t < steps; t += 2) {
+      step(a0, b0, a1, b1, t);
+      if (t + 1 < steps) step(a1, b1, a0, b0, t + 1);
+    }
   }
 
   // ---- epilogue: lane (i, g) holds columns 4 g .. 4 g + 3 of row i of every 16 x 16 tile ----
@@ -567,7 +622,8 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
     mt = (a.S + BM - 1) / BM + a.E + (a.zero_rest ? 2 : 0);
     mt = mt < a.S ? mt : a.S;
   }
-  const int64_t blocks = OP == kWgrad ? mt * nt * a.E : mt * nt;
+  // whole rounds over the 8 XCDs (workgroups are dealt to them in turn)
+  const int64_t blocks = (mt * nt + 7) / 8 * 8 * (OP == kWgrad ? a.E : 1);
   if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
   hipLaunchKernelGGL((grouped_fast_k<DT, OP, BM, BN, WM, WN>), dim3((uint32_t)blocks), dim3(64 * WM * WN), 0, s, a,
                      (int)mt, nt);
