@@ -269,13 +269,17 @@ template <int IMM>
 __device__ __forceinline__ void gg_dma(__amdgpu_buffer_rsrc_t r, char* lds, uint32_t vo, uint32_t so) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (gg_lptr)lds, 16, vo, so, IMM, 0);
 }
-// 16-B chunk swizzles of a 128-B LDS row: row-major operands (rows of 64
-// reduction elements) and transposed ones (64 reduction rows of 64 columns).
-__device__ __forceinline__ int gg_swz(int r) { return (r >> 1) & 7; }
-__device__ __forceinline__ int gg_swz_tr(int r) { return 2 * (((r >> 1) & 1) | (((r >> 3) & 1) << 1)); }
+// LDS image of one 64-deep step of an operand, 1-KiB pieces of 8 rows x 128 B:
+//   row-major   rows of 64 reduction elements; row r lies at 64 (r / 64) + 8 (r % 8) + r / 8 % 8
+//   transposed  per 64 columns, 64 reduction rows of them; row r lies at 8 (r % 8) + r / 8
+// so the 8 rows of one LDS-DMA instruction are 8 rows apart in memory: adjacent
+// rows of some power-of-two strides (8 KiB among them) fall on one cache channel,
+// 35 B/clk a CU instead of 52.  16-B chunks are XORed with a function of the LDS
+// row, so fragment reads touch every bank once.
+__device__ __forceinline__ int gg_swz(int pos) { return (pos >> 3) & 7; }
+__device__ __forceinline__ int gg_swz_tr(int pos) { return 2 * (((pos >> 1) & 1) | (((pos >> 3) & 1) << 1)); }
 
-// One operand of the product as a stream of 64-deep steps into LDS images.
-// TR false: R rows of 128 B; TR true: R / 64 images of [64][128 B].
+// One operand of the product as a stream of 64-deep steps.
 template <int R, int WAVES, bool TR>
 struct GgOperand {
   static constexpr int kPieces = R / 8 / WAVES;  // 1-KiB pieces of a step, a wave
@@ -284,51 +288,68 @@ struct GgOperand {
   int64_t step;    // bytes the base moves a step (TR)
   uint32_t vo[kPieces];
   int c8;          // !TR: this lane's first element in a step
+  gg_u4 rs;
+  uint32_t so;
 
-  __device__ __forceinline__ void issue(char* lds, int t, int w, int left) {
+  __device__ __forceinline__ void first() {
+    const int64_t b = reinterpret_cast<int64_t>(base);
+    const int64_t n = bytes < 0 ? 0 : (bytes > kGgSpan ? kGgSpan : bytes);
+    rs = gg_u4{(uint32_t)b, (uint32_t)((uint64_t)b >> 32) & 0xffffu, (uint32_t)n, 0x00020000u};
+    so = 0;
+  }
+  __device__ __forceinline__ void next() {
     if constexpr (!TR) {
-      const __amdgpu_buffer_rsrc_t r = gg_rsrc(base, bytes);
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j)  // a reduction tail reads 0
-        gg_dma<0>(r, lds + (w + WAVES * j) * 1024, c8 < left ? vo[j] : kGgOob, (uint32_t)t * 128u);
+      so += 128;
     } else {
-      const __amdgpu_buffer_rsrc_t r = gg_rsrc(base + t * step, bytes - t * step);
-#pragma unroll
-      for (int j = 0; j < kPieces; ++j) {
-        const int piece = w + WAVES * j;  // row group piece & 7 of image piece >> 3
-        gg_dma<0>(r, lds + ((piece >> 3) * 8 + (piece & 7)) * 1024, vo[j], 0);
-      }
+      base += step;
+      bytes -= step;
+      first();
     }
+  }
+  __device__ __forceinline__ void tail(int left) {  // a row-major step that ends inside, or is none: zeros
+    if constexpr (!TR) {
+#pragma unroll
+      for (int j = 0; j < kPieces; ++j) vo[j] = c8 < left ? vo[j] : kGgOob;
+    }
+  }
+  // The LDS-DMA is opaque to the compiler: it would wait for every one in
+  // flight before any LDS read.  Arrival is waited for by count (arrived()).
+  __device__ __forceinline__ void issue(uint32_t lds, int j) {
+    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(vo[j]), "s"(rs),
+                 "s"(so), "i"(WAVES * j * 1024)
+                 : "m0", "scc");
   }
 };
 
-template <int DT, bool TR, int NF>
-struct GgFrags {
-  gg_u4 v[NF];
-  // fragments of 16 rows (columns when TR) each, from wbase on; h: half of the 64-deep step
-  __device__ __forceinline__ void load(const char* lds, int wbase, int h, int lane) {
+// Fragments of 16 rows (columns when TR): lane (i, g) holds reduction elements
+// 32 h + 8 g .. + 7 of row i.  Lane part of the address; the rest is constant.
+template <bool TR>
+struct GgReader {
+  uint32_t p[TR ? 4 : 2];
+  __device__ __forceinline__ void init(int wbase, int lane) {
+    const int i = lane & 15, g = lane >> 4;
     if constexpr (!TR) {
-      const int i = lane & 15, g = lane >> 4;
-      const char* p = lds + (wbase + i) * 128 + 16 * ((4 * h + g) ^ gg_swz(i));
+      const int pos = 64 * (wbase >> 6) + 8 * (i & 7) + ((wbase & 63) >> 3) + (i >> 3);
 #pragma unroll
-      for (int x = 0; x < NF; ++x) v[x] = *reinterpret_cast<const gg_u4*>(p + x * 2048);
+      for (int h = 0; h < 2; ++h) p[h] = pos * 128 + 16 * ((4 * h + g) ^ gg_swz(pos));
     } else {
-      const int g = lane >> 4, q = (lane & 15) >> 2, pp = lane & 3;
-      const int r0 = 32 * h + 8 * g + q;
+      const int q = i >> 2, pp = i & 3, pos = 8 * q + g;  // + 4 h, + 32 for elements 4 .. 7
 #pragma unroll
-      for (int x = 0; x < NF; ++x) {
-        const int col = wbase + 16 * x;
-        const char* img = lds + (col >> 6) * 8192;
-        const int chunk = ((col & 63) >> 3) + (pp >> 1);
-        const char* a = img + r0 * 128 + 16 * (chunk ^ gg_swz_tr(r0)) + 8 * (pp & 1);
-        const gg_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(a));
-        const gg_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(a + 512));
-        const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-        v[x] = gg_u4{l2.x, l2.y, h2.x, h2.y};
-      }
+      for (int x = 0; x < 4; ++x)
+        p[x] = (wbase >> 6) * 8192 + pos * 128 + 16 * ((2 * (((wbase & 63) >> 4) ^ x) + (pp >> 1)) ^ gg_swz_tr(pos)) + 8 * (pp & 1);
     }
   }
 };
+typedef __attribute__((address_space(3))) const gg_u4* gg_lu4;
+template <bool TR>
+__device__ __forceinline__ gg_u4 gg_frag(const GgReader<TR>& rd, uint32_t img, int h, int x) {
+  if constexpr (!TR) return *(gg_lu4)(uintptr_t)(rd.p[h] + img + (x >> 2) * 8192 + (x & 3) * 256);
+  const uint32_t a = rd.p[x & 3] + img + (x >> 2) * 8192 + h * 512;
+  const gg_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(uintptr_t)(a));
+  const gg_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(uintptr_t)(a + 4096));
+  const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+  return gg_u4{l2.x, l2.y, h2.x, h2.y};
+}
 
 template <int DT>
 __device__ __forceinline__ f32x4 gg_mfma(gg_u4 a, gg_u4 b, f32x4 c) {
@@ -346,22 +367,41 @@ __device__ __forceinline__ uint32_t gg_pack2(float a, float b) {  // round to ne
   }
 }
 
-// Tile `pos` of an mt x nt grid, in strips of 4 row tiles: neighbours in this
-// order share operands, so a part of it that runs at once on one XCD (32
-// workgroups: 4 x 8 tiles) reads each of them into its L2 once.
+// Order of an mt x nt grid of tiles.  Workgroups are dealt to the 8 XCDs in
+// turn, 32 CUs each, so 256 run at once: 32 consecutive positions are one XCD's
+// share of that (4 x 8 tiles: 12 operand panels into its L2 instead of 64), and
+// 8 such shares lie together (16 x 16 tiles), so panels that several XCDs read
+// come out of the last-level cache.
+__device__ __forceinline__ int gg_pos(int b, int all) {
+  const int x = b & 7, j = b >> 3, round = j >> 5, in = j & 31;
+  const int left = all - 256 * round;
+  if (left >= 256) return 256 * round + 32 * x + in;
+  const int share = (left + 7) >> 3;  // the last round: as even as can be
+  const int pos = share * x + in;
+  return in < share && pos < left ? 256 * round + pos : -1;
+}
 __device__ __forceinline__ void gg_order(int pos, int mt, int nt, int& mi, int& ni) {
-  const int strip = pos / (4 * nt), r = pos - strip * 4 * nt;
-  const int h = mt - 4 * strip < 4 ? mt - 4 * strip : 4;
-  ni = r / h;
-  mi = 4 * strip + (r - ni * h);
+  const int strip = pos / (16 * nt);
+  int r = pos - strip * 16 * nt;
+  const int h = mt - 16 * strip < 16 ? mt - 16 * strip : 16;
+  const int nb = r / (8 * h), wd = nt - 8 * nb < 8 ? nt - 8 * nb : 8;
+  r -= nb * 8 * h;
+  const int ms = r / (4 * wd), hm = h - 4 * ms < 4 ? h - 4 * ms : 4;
+  r -= ms * 4 * wd;
+  ni = r / hm;
+  mi = 16 * strip + 4 * ms + (r - ni * hm);
+  ni += 8 * nb;
 }
 
 // BM x BN tile, WM x WN waves.
 template <int DT, int OP, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a, int mt_max, int nt) {
+__global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(GroupedArgs a, int mt_max, int nt) {
   constexpr int W = WM * WN, XF = BM / WM / 16, YF = BN / WN / 16;
   constexpr bool TA = OP == kWgrad, TB = OP != kLinear;
-  __shared__ __attribute__((aligned(1024))) char a0[BM * 128], b0[BN * 128], a1[BM * 128], b1[BN * 128];
+  // units of 256 rows x 64: A of step t, B of step t, A of step t + 1, ...
+  static_assert(BM == BN, "one unit size");
+  constexpr uint32_t kUnit = BM * 128, kUnits = 5;
+  __shared__ __attribute__((aligned(1024))) char lds[kUnits * kUnit];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rr = lane >> 3, p = lane & 7;
   const char* A = static_cast<const char*>(a.a);
@@ -374,13 +414,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
   int red;                // reduction length
   int n0;
   if constexpr (OP == kWgrad) {
-    // an expert's tiles, each XCD a contiguous part of them
-    const int per = mt_max * nt, chunk = (per + 7) / 8;
-    const int r = blockIdx.x % (8 * chunk), pos = (r & 7) * chunk + (r >> 3);
-    if (pos >= per) return;
-    e = blockIdx.x / (8 * chunk);
+    const int per = mt_max * nt, pos = gg_pos(blockIdx.x, per * a.E);
+    if (pos < 0) return;
+    e = pos / per;
     int mi, ni;
-    gg_order(pos, mt_max, nt, mi, ni);
+    gg_order(pos - e * per, mt_max, nt, mi, ni);
     m0 = (int64_t)mi * BM;
     n0 = ni * BN;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
@@ -389,11 +427,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
   } else {
     int ni = 0;
     const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
-      const int64_t all = (int64_t)mts * nt, chunk = (all + 7) / 8;
-      const int64_t pos = (blockIdx.x & 7) * chunk + (blockIdx.x >> 3);
-      if ((blockIdx.x >> 3) >= chunk || pos >= all) return -1;
+      const int pos = gg_pos(blockIdx.x, mts * nt);
+      if (pos < 0) return -1;
       int mi;
-      gg_order((int)pos, mts, nt, mi, ni);
+      gg_order(pos, mts, nt, mi, ni);
       return mi;
     });
     if (t.e == -2) return;
@@ -409,13 +446,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
   GgOperand<BM, W, TA> oa;
   GgOperand<BN, W, TB> ob;
   if constexpr (!TA) {
-    oa.c8 = 8 * (p ^ gg_swz(8 * w + rr));
+    oa.c8 = 8 * (p ^ gg_swz(8 * w));
     const bool gather = OP == kLinear && a.rows;
     oa.base = gather ? A : A + m0 * a.lda * 2;
     oa.bytes = gather ? ((a.T - 1) * a.lda + a.K) * 2 : ((int64_t)(mrows - 1) * a.lda + red) * 2;
 #pragma unroll
     for (int j = 0; j < oa.kPieces; ++j) {
-      const int r = 8 * (w + W * j) + rr;
+      const int r = 64 * (W * j / 8) + w + 8 * rr;
       int64_t row = r;
       bool ok = r < mrows;
       if (gather) {
@@ -425,33 +462,33 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
       oa.vo[j] = ok ? (uint32_t)((row * a.lda + oa.c8) * 2) : kGgOob;
     }
   } else {
-    const int r = 8 * (w & 7) + rr;
+    const int r = w + 8 * rr;
     oa.base = A + (red0 * a.lda + m0) * 2;
     oa.bytes = ((int64_t)(red - 1) * a.lda + mrows) * 2;
     oa.step = 64 * a.lda * 2;
 #pragma unroll
     for (int j = 0; j < oa.kPieces; ++j) {
-      const int c = 64 * ((w + W * j) >> 3) + 8 * (p ^ gg_swz_tr(r));
+      const int c = 64 * (W * j / 8) + 8 * (p ^ gg_swz_tr(8 * w + rr));
       oa.vo[j] = c < mrows ? (uint32_t)((r * a.lda + c) * 2) : kGgOob;
     }
   }
   if constexpr (!TB) {
-    ob.c8 = 8 * (p ^ gg_swz(8 * w + rr));
+    ob.c8 = 8 * (p ^ gg_swz(8 * w));
     ob.base = B + ((int64_t)e * a.strb + (int64_t)n0 * a.ldb) * 2;
     ob.bytes = ((int64_t)(ncols - 1) * a.ldb + red) * 2;
 #pragma unroll
     for (int j = 0; j < ob.kPieces; ++j) {
-      const int r = 8 * (w + W * j) + rr;
+      const int r = 64 * (W * j / 8) + w + 8 * rr;
       ob.vo[j] = r < ncols ? (uint32_t)((r * a.ldb + ob.c8) * 2) : kGgOob;
     }
   } else {
-    const int r = 8 * (w & 7) + rr;
+    const int r = w + 8 * rr;
     ob.base = OP == kDgrad ? B + ((int64_t)e * a.strb + n0) * 2 : B + (red0 * a.ldb + n0) * 2;
     ob.bytes = ((int64_t)(red - 1) * a.ldb + ncols) * 2;
     ob.step = 64 * a.ldb * 2;
 #pragma unroll
     for (int j = 0; j < ob.kPieces; ++j) {
-      const int c = 64 * ((w + W * j) >> 3) + 8 * (p ^ gg_swz_tr(r));
+      const int c = 64 * (W * j / 8) + 8 * (p ^ gg_swz_tr(8 * w + rr));
       ob.vo[j] = c < ncols ? (uint32_t)((r * a.ldb + c) * 2) : kGgOob;
     }
   }
@@ -468,60 +505,90 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
     for (int y = 0; y < YF; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
   const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
 
-  // Fragments of the step's two halves are kept apart, so a half's MFMAs run
-  // while the next half's LDS reads are in flight.  One barrier a step, between
-  // the halves: every wave has then read all of this step (its buffer may be
-  // filled with step t + 2) and step t + 1 has arrived.
+  // A step has two halves of 32 deep.  A half's MFMAs run on fragments in
+  // registers while the next half's are read from LDS and 32 KiB of a later step
+  // arrive (first half: A of step t + 2, second: B), all spread over the half so
+  // that nothing queues: LDS-DMA moves 52 B/clk a CU, half of what the step takes.
+  // One barrier a step, between its halves: everybody has read all of step t, so
+  // its units may be filled, and step t + 1 is in LDS.
+  static_assert(W == 8, "piece maps");
   const int steps = (red + 63) / 64;
-  GgFrags<DT, TA, XF> fa0, fa1;
-  GgFrags<DT, TB, YF> fb0, fb1;
-  auto mma = [&](const GgFrags<DT, TA, XF>& fa, const GgFrags<DT, TB, YF>& fb) {
-#pragma unroll
-    for (int x = 0; x < XF; ++x)
-#pragma unroll
-      for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(fb.v[y], fa.v[x], acc[x][y]);
-    // one LDS read, then the MFMAs that hide it
-    constexpr int kReads = XF * (TA ? 2 : 1) + YF * (TB ? 2 : 1), kEach = XF * YF / kReads > 0 ? XF * YF / kReads : 1;
-#pragma unroll
-    for (int q = 0; q < kReads; ++q) {
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, kEach, 0);
-    }
+  constexpr int kPA = GgOperand<BM, W, TA>::kPieces, kPB = GgOperand<BN, W, TB>::kPieces;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
+  asm volatile("" ::"v"(lds0) : "memory");
+  GgReader<TA> ra;
+  GgReader<TB> rb;
+  ra.init(wm, lane);
+  rb.init(wn, lane);
+  const uint32_t dma0 = lds0 + w * 1024;
+  gg_u4 fa[2][XF], fb[2][YF];
+  auto turn = [&](uint32_t u) {  // unit offset, wrapped
+    const uint32_t v = u - kUnits * kUnit;
+    return u < v ? u : v;
   };
-  auto arrived = [&]() {  // this wave's pieces are in LDS and its reads done, then everybody's
+  auto sync = [&]() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    __builtin_amdgcn_s_waitcnt(0x0070 | kPA);  // lgkmcnt(0), vmcnt(kPA): all but the newest unit
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  auto stage = [&](char* la, char* lb, int t) {
-    if (t < steps) {
-      oa.issue(la, t, w, red - 64 * t);
-      ob.issue(lb, t, w, red - 64 * t);
+  // MFMAs on (ac, bc); read half h of images (ia, ib) into (an, bn)
+  auto half = [&](auto& op, uint32_t dst, int h, uint32_t ia, uint32_t ib, gg_u4 (&ac)[XF], gg_u4 (&bc)[YF], gg_u4 (&an)[XF],
+                  gg_u4 (&bn)[YF], int left) {
+    constexpr int kR = XF + YF, kOver = XF - 2;
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      if (x == 1) {
+        op.next();
+        if (left < 64) op.tail(left);
+      }
+#pragma unroll
+      for (int q = 0; q < kR; ++q)
+        if (q * kOver / kR == x) {
+          if (q < YF) bn[q] = gg_frag<TB>(rb, ib, h, q);
+          else an[q - YF] = gg_frag<TA>(ra, ia, h, q - YF);
+        }
+      if (x & 1) op.issue(dst, x / 2);
+#pragma unroll
+      for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(bc[y], ac[x], acc[x][y]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto step = [&](char* ca, char* cb, const char* na, const char* nb, int t) {
-    fa1.load(ca, wm, 1, lane);
-    fb1.load(cb, wn, 1, lane);
-    mma(fa0, fb0);
-    arrived();
-    stage(ca, cb, t + 2);
-    fa0.load(na, wm, 0, lane);
-    fb0.load(nb, wn, 0, lane);
-    mma(fa1, fb1);
-    __builtin_amdgcn_sched_barrier(0);
-  };
+  static_assert(XF == 8 && kPA == 4 && kPB == 4, "four LDS-DMA instructions a half");
   if (steps > 0) {
-    stage(a0, b0, 0);
-    arrived();
-    stage(a1, b1, 1);
-    fa0.load(a0, wm, 0, lane);
-    fb0.load(b0, wn, 0, lane);
-    for (int t = 0; t < steps; t += 2) {
-      step(a0, b0, a1, b1, t);
-      if (t + 1 < steps) step(a1, b1, a0, b0, t + 1);
+    oa.first();
+    ob.first();
+    if (red < 64) { oa.tail(red); ob.tail(red); }
+#pragma unroll
+    for (int j = 0; j < kPA; ++j) oa.issue(dma0, j);
+#pragma unroll
+    for (int j = 0; j < kPB; ++j) ob.issue(dma0 + kUnit, j);
+    oa.next();
+    ob.next();
+    if (red < 128) { oa.tail(red - 64); ob.tail(red - 64); }
+#pragma unroll
+    for (int j = 0; j < kPA; ++j) oa.issue(dma0 + 2 * kUnit, j);
+#pragma unroll
+    for (int j = 0; j < kPB; ++j) ob.issue(dma0 + 3 * kUnit, j);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070 | (kPA + kPB));
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int y = 0; y < YF; ++y) fb[0][y] = gg_frag<TB>(rb, lds0 + kUnit, 0, y);
+#pragma unroll
+    for (int x = 0; x < XF; ++x) fa[0][x] = gg_frag<TA>(ra, lds0, 0, x);
+    uint32_t ua = 0;
+    for (int t = 0; t < steps; ++t) {
+      const int left = red - 64 * (t + 2);
+      const uint32_t ub = turn(ua + kUnit), va = turn(ua + 2 * kUnit), vb = turn(va + kUnit), fr = turn(vb + kUnit);
+      half(oa, dma0 + fr, 1, lds0 + ua, lds0 + ub, fa[0], fb[0], fa[1], fb[1], left);
+      sync();
+      half(ob, dma0 + ua, 0, lds0 + va, lds0 + vb, fa[1], fb[1], fa[0], fb[0], left);
+      ua = va;
     }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // no LDS-DMA outlives the workgroup
   }
 
   // ---- epilogue: lane (i, g) holds columns 4 g .. 4 g + 3 of row i of every 16 x 16 tile ----
@@ -622,9 +689,8 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
     mt = (a.S + BM - 1) / BM + a.E + (a.zero_rest ? 2 : 0);
     mt = mt < a.S ? mt : a.S;
   }
-  // whole rounds over the 8 XCDs (workgroups are dealt to them in turn)
-  const int64_t blocks = (mt * nt + 7) / 8 * 8 * (OP == kWgrad ? a.E : 1);
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  const int64_t tiles = mt * nt * (OP == kWgrad ? a.E : 1), blocks = (tiles + 7) / 8 * 8;  // the XCDs in turn
+  if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
   hipLaunchKernelGGL((grouped_fast_k<DT, OP, BM, BN, WM, WN>), dim3((uint32_t)blocks), dim3(64 * WM * WN), 0, s, a,
                      (int)mt, nt);
   return hipGetLastError();
