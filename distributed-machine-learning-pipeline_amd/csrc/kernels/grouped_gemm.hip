@@ -10,11 +10,21 @@
 // workgroup finds its expert by a wave scan over the groups' tile counts.
 // Offsets and rows are clamped to the buffers they index: a wrong plan gives
 // wrong numbers, never an access outside the operands.
+#include <type_traits>
+
 #include "common.h"
 #include "../dsml.h"
 #include "../experts.h"
 
+// The LDS-DMA below sets M0 by itself; the compiler keeps nothing there.
+#pragma clang diagnostic ignored "-Winline-asm"
+
 namespace dsml {
+
+typedef int gg_i4 __attribute__((ext_vector_type(4)));
+// A scalar load behind a buffer descriptor (0 past its end).
+__device__ int gg_sload(gg_i4 rsrc, int offset, int policy) __asm("llvm.amdgcn.s.buffer.load.i32");
+
 namespace {
 
 typedef __bf16 gg_bf16x8 __attribute__((ext_vector_type(8)));
@@ -279,8 +289,10 @@ __device__ __forceinline__ void gg_dma(__amdgpu_buffer_rsrc_t r, char* lds, uint
 __device__ __forceinline__ int gg_swz(int pos) { return (pos >> 3) & 7; }
 __device__ __forceinline__ int gg_swz_tr(int pos) { return 2 * (((pos >> 1) & 1) | (((pos >> 3) & 1) << 1)); }
 
-// One operand of the product as a stream of 64-deep steps.
-template <int R, int WAVES, bool TR>
+// One operand of the product as a stream of 64-deep steps.  GATHER (transposed
+// only): reduction row k is row ids[k] of base; a step's 8 ids of a wave are
+// scalar loads made a step ahead.
+template <int R, int WAVES, bool TR, bool GATHER = false>
 struct GgOperand {
   static constexpr int kPieces = R / 8 / WAVES;  // 1-KiB pieces of a step, a wave
   const char* base;
@@ -290,6 +302,26 @@ struct GgOperand {
   int c8;          // !TR: this lane's first element in a step
   gg_u4 rs;
   uint32_t so;
+  // GATHER
+  gg_i4 irs;        // the group's ids
+  uint32_t iat;     // byte offset of this wave's first id of the step to fetch
+  int id[8];
+  uint32_t ld2, rows, rowoff;
+  int k, rr;        // this lane's reduction row in a step: w + 8 rr
+
+  __device__ __forceinline__ void fetch_ids() {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) id[q] = gg_sload(irs, (int)(iat + 32 * q), 0);
+    iat += 256;
+  }
+  // Row offset of the step whose ids were fetched (left: its reduction rows); fetches the next ids.
+  __device__ __forceinline__ void take_ids(int left) {
+    int v = id[0];
+#pragma unroll
+    for (int q = 1; q < 8; ++q) v = rr == q ? id[q] : v;
+    rowoff = (uint32_t)v < rows && k < left ? (uint32_t)v * ld2 : kGgOob;
+    fetch_ids();
+  }
 
   __device__ __forceinline__ void first() {
     const int64_t b = reinterpret_cast<int64_t>(base);
@@ -309,13 +341,24 @@ struct GgOperand {
   __device__ __forceinline__ void tail(int left) {  // a row-major step that ends inside, or is none: zeros
     if constexpr (!TR) {
 #pragma unroll
-      for (int j = 0; j < kPieces; ++j) vo[j] = c8 < left ? vo[j] : kGgOob;
+      for (int j = 0; j < kPieces; ++j) vo[j] = (c8 ^ (8 * (WAVES * j & 7))) < left ? vo[j] : kGgOob;
+    }
+  }
+  // On to the next step, which has `left` reduction rows or elements (or fewer than none).
+  __device__ __forceinline__ void advance(int left) {
+    if constexpr (GATHER) {
+      take_ids(left);
+    } else {
+      next();
+      if (left < 64) tail(left);
     }
   }
   // The LDS-DMA is opaque to the compiler: it would wait for every one in
   // flight before any LDS read.  Arrival is waited for by count (arrived()).
   __device__ __forceinline__ void issue(uint32_t lds, int j) {
-    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(vo[j]), "s"(rs),
+    uint32_t v = vo[j];
+    if constexpr (GATHER) v = __builtin_elementwise_add_sat(v, rowoff);  // kGgOob stays past the end
+    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(v), "s"(rs),
                  "s"(so), "i"(WAVES * j * 1024)
                  : "m0", "scc");
   }
@@ -356,6 +399,12 @@ __device__ __forceinline__ f32x4 gg_mfma(gg_u4 a, gg_u4 b, f32x4 c) {
   return gg_mfma16<DT>(__builtin_bit_cast(uint4, a), __builtin_bit_cast(uint4, b), c);
 }
 
+// This wave's LDS reads are done, and its vector-memory operations but the last N.
+template <int N>
+__device__ __forceinline__ void gg_wait() {
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
+}
+
 template <int DT>
 __device__ __forceinline__ uint32_t gg_pack2(float a, float b) {  // round to nearest even
   if constexpr (DT == kBF16) {
@@ -394,7 +443,7 @@ __device__ __forceinline__ void gg_order(int pos, int mt, int nt, int& mi, int& 
 }
 
 // BM x BN tile, WM x WN waves.
-template <int DT, int OP, int BM, int BN, int WM, int WN>
+template <int DT, int OP, int BM, int BN, int WM, int WN, bool GATHER>
 __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(GroupedArgs a, int mt_max, int nt) {
   constexpr int W = WM * WN, XF = BM / WM / 16, YF = BN / WN / 16;
   constexpr bool TA = OP == kWgrad, TB = OP != kLinear;
@@ -422,8 +471,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     m0 = (int64_t)mi * BM;
     n0 = ni * BN;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
-    red0 = gg_clamp(a.offsets[e], 0, a.S);
-    red = (int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0);
+    red0 = __builtin_amdgcn_readfirstlane((int)gg_clamp(a.offsets[e], 0, a.S));
+    red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
   } else {
     int ni = 0;
     const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
@@ -444,7 +493,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
 
   // ---- operand streams ----
   GgOperand<BM, W, TA> oa;
-  GgOperand<BN, W, TB> ob;
+  GgOperand<BN, W, TB, GATHER> ob;
   if constexpr (!TA) {
     oa.c8 = 8 * (p ^ gg_swz(8 * w));
     const bool gather = OP == kLinear && a.rows;
@@ -452,23 +501,22 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     oa.bytes = gather ? ((a.T - 1) * a.lda + a.K) * 2 : ((int64_t)(mrows - 1) * a.lda + red) * 2;
 #pragma unroll
     for (int j = 0; j < oa.kPieces; ++j) {
-      const int r = 64 * (W * j / 8) + w + 8 * rr;
+      const int r = 64 * (W * j / 8) + (w + W * j % 8) + 8 * rr, c = oa.c8 ^ (8 * (W * j % 8));
       int64_t row = r;
       bool ok = r < mrows;
       if (gather) {
         row = ok && e >= 0 ? a.rows[m0 + r] : 0;
         ok = ok && row >= 0 && row < a.T;
       }
-      oa.vo[j] = ok ? (uint32_t)((row * a.lda + oa.c8) * 2) : kGgOob;
+      oa.vo[j] = ok ? (uint32_t)((row * a.lda + c) * 2) : kGgOob;
     }
   } else {
-    const int r = w + 8 * rr;
     oa.base = A + (red0 * a.lda + m0) * 2;
     oa.bytes = ((int64_t)(red - 1) * a.lda + mrows) * 2;
     oa.step = 64 * a.lda * 2;
 #pragma unroll
     for (int j = 0; j < oa.kPieces; ++j) {
-      const int c = 64 * (W * j / 8) + 8 * (p ^ gg_swz_tr(8 * w + rr));
+      const int r = (w + W * j % 8) + 8 * rr, c = 64 * (W * j / 8) + 8 * (p ^ gg_swz_tr(8 * w + rr));
       oa.vo[j] = c < mrows ? (uint32_t)((r * a.lda + c) * 2) : kGgOob;
     }
   }
@@ -478,17 +526,25 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     ob.bytes = ((int64_t)(ncols - 1) * a.ldb + red) * 2;
 #pragma unroll
     for (int j = 0; j < ob.kPieces; ++j) {
-      const int r = 64 * (W * j / 8) + w + 8 * rr;
-      ob.vo[j] = r < ncols ? (uint32_t)((r * a.ldb + ob.c8) * 2) : kGgOob;
+      const int r = 64 * (W * j / 8) + (w + W * j % 8) + 8 * rr, c = ob.c8 ^ (8 * (W * j % 8));
+      ob.vo[j] = r < ncols ? (uint32_t)((r * a.ldb + c) * 2) : kGgOob;
     }
   } else {
-    const int r = w + 8 * rr;
-    ob.base = OP == kDgrad ? B + ((int64_t)e * a.strb + n0) * 2 : B + (red0 * a.ldb + n0) * 2;
-    ob.bytes = ((int64_t)(red - 1) * a.ldb + ncols) * 2;
+    ob.base = OP == kDgrad ? B + ((int64_t)e * a.strb + n0) * 2 : B + ((GATHER ? 0 : red0 * a.ldb) + n0) * 2;
+    ob.bytes = ((GATHER ? a.T - 1 : (int64_t)(red - 1)) * a.ldb + ncols) * 2;
     ob.step = 64 * a.ldb * 2;
+    if constexpr (GATHER) {
+      const int64_t ip = gg_uni(reinterpret_cast<int64_t>(a.rows + red0));
+      ob.irs = gg_i4{(int)ip, (int)(ip >> 32) & 0xffff, 4 * red, 0x00020000};
+      ob.iat = 4 * w;
+      ob.ld2 = (uint32_t)a.ldb * 2;
+      ob.rows = (uint32_t)a.T;
+      ob.rr = rr;
+      ob.k = w + 8 * rr;
+    }
 #pragma unroll
     for (int j = 0; j < ob.kPieces; ++j) {
-      const int c = 64 * (W * j / 8) + 8 * (p ^ gg_swz_tr(8 * w + rr));
+      const int r = GATHER ? 0 : (w + W * j % 8) + 8 * rr, c = 64 * (W * j / 8) + 8 * (p ^ gg_swz_tr(8 * w + rr));
       ob.vo[j] = c < ncols ? (uint32_t)((r * a.ldb + c) * 2) : kGgOob;
     }
   }
@@ -511,9 +567,9 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   // that nothing queues: LDS-DMA moves 52 B/clk a CU, half of what the step takes.
   // One barrier a step, between its halves: everybody has read all of step t, so
   // its units may be filled, and step t + 1 is in LDS.
-  static_assert(W == 8, "piece maps");
+  static_assert(W == 8 || W == 4, "piece maps");
   const int steps = (red + 63) / 64;
-  constexpr int kPA = GgOperand<BM, W, TA>::kPieces, kPB = GgOperand<BN, W, TB>::kPieces;
+  constexpr int kPA = GgOperand<BM, W, TA>::kPieces, kPB = GgOperand<BN, W, TB, GATHER>::kPieces;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
   asm volatile("" ::"v"(lds0) : "memory");
   GgReader<TA> ra;
@@ -522,13 +578,19 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   rb.init(wn, lane);
   const uint32_t dma0 = lds0 + w * 1024;
   gg_u4 fa[2][XF], fb[2][YF];
+  const bool sums = OP == kWgrad && a.db && n0 == 0;
+  constexpr uint32_t kOnes = DT == kBF16 ? 0x3f803f80u : 0x3c003c00u;
+  const gg_u4 ones = {kOnes, kOnes, kOnes, kOnes};
+  f32x4 accs[XF / WN > 0 ? XF / WN : 1];
+#pragma unroll
+  for (int u = 0; u < XF / WN; ++u) accs[u] = {0.f, 0.f, 0.f, 0.f};
   auto turn = [&](uint32_t u) {  // unit offset, wrapped
     const uint32_t v = u - kUnits * kUnit;
     return u < v ? u : v;
   };
   auto sync = [&]() {
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | kPA);  // lgkmcnt(0), vmcnt(kPA): all but the newest unit
+    gg_wait<kPA>();  // all but the newest unit
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -537,11 +599,13 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   auto half = [&](auto& op, uint32_t dst, int h, uint32_t ia, uint32_t ib, gg_u4 (&ac)[XF], gg_u4 (&bc)[YF], gg_u4 (&an)[XF],
                   gg_u4 (&bn)[YF], int left) {
     constexpr int kR = XF + YF, kOver = XF - 2;
+    if constexpr (GATHER) {  // before this half's LDS reads: the scalar loads share their counter
+      if constexpr (std::is_same_v<std::decay_t<decltype(op)>, GgOperand<BN, W, TB, true>>) op.advance(left);
+    }
 #pragma unroll
     for (int x = 0; x < XF; ++x) {
       if (x == 1) {
-        op.next();
-        if (left < 64) op.tail(left);
+        if constexpr (!GATHER || !std::is_same_v<std::decay_t<decltype(op)>, GgOperand<BN, W, TB, true>>) op.advance(left);
       }
 #pragma unroll
       for (int q = 0; q < kR; ++q)
@@ -549,30 +613,48 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
           if (q < YF) bn[q] = gg_frag<TB>(rb, ib, h, q);
           else an[q - YF] = gg_frag<TA>(ra, ia, h, q - YF);
         }
-      if (x & 1) op.issue(dst, x / 2);
+#pragma unroll
+      for (int j = 0; j < kPA; ++j)  // all after next()
+        if (1 + j * (XF - 1) / kPA == x) op.issue(dst, j);
 #pragma unroll
       for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(bc[y], ac[x], acc[x][y]);
       __builtin_amdgcn_sched_barrier(0);
     }
+    if constexpr (OP == kWgrad) {
+      if (sums) {  // column sums of dz: a product with ones, each wave of a row its part
+#pragma unroll
+        for (int c = 0; c < WN; ++c)
+          if (w % WN == c) {
+#pragma unroll
+            for (int u = 0; u < XF / WN; ++u) accs[u] = gg_mfma<DT>(ones, ac[XF / WN * c + u], accs[u]);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
   };
-  static_assert(XF == 8 && kPA == 4 && kPB == 4, "four LDS-DMA instructions a half");
+  static_assert(kPA == kPB, "one count for both operands");
   if (steps > 0) {
     oa.first();
     ob.first();
-    if (red < 64) { oa.tail(red); ob.tail(red); }
+    if (red < 64) oa.tail(red);
+    if constexpr (GATHER) {
+      ob.fetch_ids();
+      ob.take_ids(red);
+    } else if (red < 64) {
+      ob.tail(red);
+    }
 #pragma unroll
     for (int j = 0; j < kPA; ++j) oa.issue(dma0, j);
 #pragma unroll
     for (int j = 0; j < kPB; ++j) ob.issue(dma0 + kUnit, j);
-    oa.next();
-    ob.next();
-    if (red < 128) { oa.tail(red - 64); ob.tail(red - 64); }
+    oa.advance(red - 64);
+    ob.advance(red - 64);
 #pragma unroll
     for (int j = 0; j < kPA; ++j) oa.issue(dma0 + 2 * kUnit, j);
 #pragma unroll
     for (int j = 0; j < kPB; ++j) ob.issue(dma0 + 3 * kUnit, j);
     asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0x0070 | (kPA + kPB));
+    gg_wait<kPA + kPB>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
@@ -595,6 +677,13 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   const int i = lane & 15, g = lane >> 4;
   if constexpr (OP == kWgrad) {
     float* out = static_cast<float*>(a.out) + (int64_t)e * a.stro;
+    if (sums && g == 0) {
+#pragma unroll
+      for (int u = 0; u < XF / WN; ++u) {
+        const int m = wm + 16 * (XF / WN * (w % WN) + u) + i;
+        if (m < mrows) a.db[(int64_t)e * a.N + m0 + m] = accs[u][0];
+      }
+    }
 #pragma unroll
     for (int x = 0; x < XF; ++x) {
       const int m = wm + 16 * x + i;
@@ -674,12 +763,14 @@ bool fast_ok(GroupedOp op, const GroupedArgs& a) {
   if (op != kWgrad && a.E > 1 && a.strb % 8) return false;
   if (a.lda > 0x7fffff || a.ldb > 0x7fffff) return false;
   if (op == kLinear && a.rows && (a.T * a.lda + a.K) * 2 > kGgSpan) return false;
-  if (op == kWgrad) return a.rows == nullptr && a.db == nullptr && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && a.ldo % 4 == 0 && (a.E <= 1 || a.stro % 4 == 0);
+  if (op == kWgrad)
+    return (!a.rows || (a.T * a.ldb + a.K) * 2 <= kGgSpan) && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
+           a.ldo % 4 == 0 && (a.E <= 1 || a.stro % 4 == 0);
   if (!gg_al(a.out, a.ldo, 0)) return false;
   return op != kDgrad || !a.mask || gg_al(a.mask, a.ldmask, 0);
 }
 
-template <int DT, int OP, int BM, int BN, int WM, int WN>
+template <int DT, int OP, int BM, int BN, int WM, int WN, bool GATHER = false>
 hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
   const int cols = OP == kLinear ? a.N : a.K;
   const int nt = (cols + BN - 1) / BN;
@@ -691,7 +782,7 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
   }
   const int64_t tiles = mt * nt * (OP == kWgrad ? a.E : 1), blocks = (tiles + 7) / 8 * 8;  // the XCDs in turn
   if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((grouped_fast_k<DT, OP, BM, BN, WM, WN>), dim3((uint32_t)blocks), dim3(64 * WM * WN), 0, s, a,
+  hipLaunchKernelGGL((grouped_fast_k<DT, OP, BM, BN, WM, WN, GATHER>), dim3((uint32_t)blocks), dim3(64 * WM * WN), 0, s, a,
                      (int)mt, nt);
   return hipGetLastError();
 }
@@ -700,7 +791,8 @@ hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
   switch (op) {
     case kLinear: return launch_fast<DT, kLinear, 256, 256, 2, 4>(a, s);
     case kDgrad: return launch_fast<DT, kDgrad, 256, 256, 2, 4>(a, s);
-    default: return launch_fast<DT, kWgrad, 256, 256, 2, 4>(a, s);
+    default:
+      return a.rows ? launch_fast<DT, kWgrad, 256, 256, 2, 4, true>(a, s) : launch_fast<DT, kWgrad, 256, 256, 2, 4>(a, s);
   }
 }
 
