@@ -57,67 +57,106 @@ struct GgTile {
 
 __device__ __forceinline__ int64_t gg_clamp(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
-// The groups' row tiles, experts first, then (zero_rest) the tiles of the rows
-// before the first group and behind the last.  `pick` maps the number of tiles
-// to the one wanted (< 0 or too large: nothing).  One wave scan per 64 experts,
-// done by every wave for itself: no LDS, no barrier.
-template <class Pick>
-__device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, int BM, bool zero_rest, Pick pick) {
-  const int lane = threadIdx.x & 63;
-  int a = 0, b = 0, n = 0, inc = 0, tot = 0;
-  auto scan = [&](int e0) {
-    const int e = e0 + lane;
+// Inclusive sums over the lanes of a wave: within rows of 16, then across them.
+__device__ __forceinline__ int gg_scan64(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
+  return v;
+}
+
+// The groups, cut into tiles on the GPU: count(rows) is what a group of that
+// many rows holds of some kind of tile.  One wave scan per 64 experts, done by
+// every wave for itself: no LDS, no barrier.
+struct GgGroups {
+  const int32_t* off;
+  int E;
+  int64_t S;
+
+  __device__ __forceinline__ void bounds(int e, int64_t& a, int64_t& b) const {
+    a = gg_clamp(off[e], 0, S);
+    b = gg_clamp(off[e + 1], a, S);
+  }
+  template <class Count>
+  __device__ __forceinline__ void scan(int e0, Count count, int& a, int& b, int& n, int& inc) const {
+    const int lane = threadIdx.x & 63;
     a = b = 0;
-    if (e < E) {
-      a = (int)gg_clamp(off[e], 0, S);
-      b = (int)gg_clamp(off[e + 1], a, S);
+    if (e0 + lane < E) {
+      int64_t x, y;
+      bounds(e0 + lane, x, y);
+      a = (int)x;
+      b = (int)y;
     }
-    n = (int)(((int64_t)b - a + BM - 1) / BM);
-    inc = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int u = __shfl_up(inc, o);
-      if (lane >= o) inc += u;
-    }
-    tot = __builtin_amdgcn_readlane(inc, 63);
-  };
-  int total = 0;
-  for (int e0 = (E - 1) & ~63; e0 >= 0; e0 -= 64) {  // the first 64 stay in registers
-    scan(e0);
-    total += tot;
+    n = count((int64_t)b - a);
+    inc = gg_scan64(n);
   }
-  int64_t head = 0, tail = 0;
-  int hn = 0, tn = 0;
-  if (zero_rest) {
-    head = gg_clamp(off[0], 0, S);
-    tail = gg_clamp(off[E], head, S);
-    hn = (int)((head + BM - 1) / BM);
-    tn = (int)((S - tail + BM - 1) / BM);
-  }
-  GgTile t{-2, 0, 0};
-  int mt = pick(total + hn + tn);
-  if (mt < 0) return t;
-  if (mt < total) {
-    int e0 = 0;
-    while (mt >= tot) {
-      mt -= tot;
-      e0 += 64;
-      if (e0 >= E) return t;
-      scan(e0);
+  template <class Count>
+  __device__ __forceinline__ int total(Count count) const {
+    int t = 0;
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      int a, b, n, inc;
+      scan(e0, count, a, b, n, inc);
+      t += __builtin_amdgcn_readlane(inc, 63);
     }
-    const int l = __ffsll((unsigned long long)__ballot(inc > mt)) - 1;
-    const int first = __builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(n, l);
-    const int64_t a0 = __builtin_amdgcn_readlane(a, l), b0 = __builtin_amdgcn_readlane(b, l);
-    t.e = e0 + l;
-    t.s0 = a0 + (int64_t)(mt - first) * BM;
-    t.s1 = t.s0 + BM < b0 ? t.s0 + BM : b0;
     return t;
   }
-  mt -= total;
-  if (mt < hn) {
-    t.e = -1; t.s0 = (int64_t)mt * BM; t.s1 = t.s0 + BM < head ? t.s0 + BM : head;
-  } else if (mt - hn < tn) {
-    t.e = -1; t.s0 = tail + (int64_t)(mt - hn) * BM; t.s1 = t.s0 + BM < S ? t.s0 + BM : S;
+  // The group that holds tile t, its rows and the tile's number in it.
+  template <class Count>
+  __device__ __forceinline__ bool find(int t, Count count, int& e, int64_t& lo, int64_t& hi, int& in) const {
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      int a, b, n, inc;
+      scan(e0, count, a, b, n, inc);
+      const int tot = __builtin_amdgcn_readlane(inc, 63);
+      if (t < tot) {
+        const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)__ballot(inc > t)) - 1);
+        in = t - (__builtin_amdgcn_readlane(inc, l) - __builtin_amdgcn_readlane(n, l));
+        lo = __builtin_amdgcn_readlane(a, l);
+        hi = __builtin_amdgcn_readlane(b, l);
+        e = e0 + l;
+        return true;
+      }
+      t -= tot;
+    }
+    return false;
+  }
+  // Tiles of BM rows that lie in no group: before the first, behind the last.
+  __device__ __forceinline__ void rest(int& head, int& tail, int BM) const {
+    const int64_t h = gg_clamp(off[0], 0, S), t = gg_clamp(off[E], h, S);
+    head = (int)((h + BM - 1) / BM);
+    tail = (int)((S - t + BM - 1) / BM);
+  }
+  __device__ __forceinline__ bool find_rest(int t, int BM, int64_t& lo, int64_t& hi) const {
+    const int64_t h = gg_clamp(off[0], 0, S), u = gg_clamp(off[E], h, S), hn = (h + BM - 1) / BM;
+    lo = t < hn ? (int64_t)t * BM : u + (t - hn) * BM;
+    hi = t < hn ? h : S;
+    hi = lo + BM < hi ? lo + BM : hi;
+    return lo < hi;
+  }
+};
+
+// Row tile of BM rows number pick(how many there are): the experts' tiles, then
+// (zero_rest) those of the rows in no group.
+template <class Pick>
+__device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, int BM, bool zero_rest, Pick pick) {
+  const GgGroups gr{off, E, S};
+  auto count = [BM](int64_t rows) { return (int)((rows + BM - 1) / BM); };
+  const int total = gr.total(count);
+  int head = 0, tail = 0;
+  if (zero_rest) gr.rest(head, tail, BM);
+  GgTile t{-2, 0, 0};
+  const int mt = pick(total + head + tail);
+  if (mt < 0) return t;
+  if (mt < total) {
+    int64_t lo, hi;
+    int in;
+    if (!gr.find(mt, count, t.e, lo, hi, in)) return t;
+    t.s0 = lo + (int64_t)in * BM;
+    t.s1 = t.s0 + BM < hi ? t.s0 + BM : hi;
+  } else if (mt - total < head + tail && gr.find_rest(mt - total, BM, t.s0, t.s1)) {
+    t.e = -1;
   }
   return t;
 }
@@ -264,9 +303,17 @@ typedef uint32_t gg_u4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kGgOob = 0xfffffff0u;    // past every buffer: reads 0
 constexpr int64_t kGgSpan = 0xffffff00LL;   // bytes a buffer descriptor may span
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t gg_rsrc(const void* base, int64_t bytes) {
-  const uint32_t n = bytes <= 0 ? 0u : (bytes > kGgSpan ? (uint32_t)kGgSpan : (uint32_t)bytes);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, n, 0x00020000);
+__device__ __forceinline__ gg_u4 gg_desc(const char* base, int64_t bytes) {
+  const int64_t b = reinterpret_cast<int64_t>(base);
+  const int64_t n = bytes < 0 ? 0 : (bytes > kGgSpan ? kGgSpan : bytes);
+  return gg_u4{(uint32_t)b, (uint32_t)((uint64_t)b >> 32) & 0xffffu, (uint32_t)n, 0x00020000u};
+}
+// 1 KiB straight into LDS at `lds`, 16 B a lane.  Opaque to the compiler, which
+// would wait for every one in flight before any LDS read; arrival is waited for
+// by count (gg_wait).
+__device__ __forceinline__ void gg_dma(uint32_t lds, uint32_t vo, gg_u4 rs, uint32_t so) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(vo), "s"(rs), "s"(so)
+               : "m0");
 }
 // A value every lane holds, in scalar registers.
 __device__ __forceinline__ int64_t gg_uni(int64_t v) {
@@ -275,10 +322,6 @@ __device__ __forceinline__ int64_t gg_uni(int64_t v) {
   return (int64_t)(((uint64_t)hi << 32) | lo);
 }
 __device__ __forceinline__ const char* gg_uni(const char* v) { return reinterpret_cast<const char*>(gg_uni((int64_t)v)); }
-template <int IMM>
-__device__ __forceinline__ void gg_dma(__amdgpu_buffer_rsrc_t r, char* lds, uint32_t vo, uint32_t so) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (gg_lptr)lds, 16, vo, so, IMM, 0);
-}
 // LDS image of one 64-deep step of an operand, 1-KiB pieces of 8 rows x 128 B:
 //   row-major   rows of 64 reduction elements; row r lies at 64 (r / 64) + 8 (r % 8) + r / 8 % 8
 //   transposed  per 64 columns, 64 reduction rows of them; row r lies at 8 (r % 8) + r / 8
@@ -305,28 +348,36 @@ struct GgOperand {
   // GATHER
   gg_i4 irs;        // the group's ids
   uint32_t iat;     // byte offset of this wave's first id of the step to fetch
-  int id[8];
-  uint32_t ld2, rows, rowoff;
+  static constexpr int kSets = 8 / WAVES;  // rows w + 8 rr, or those and w + 4 + 8 rr
+  int id[kSets][8];
+  uint32_t ld2, rows, rowoff[kSets];
   int k, rr;        // this lane's reduction row in a step: w + 8 rr
 
   __device__ __forceinline__ void fetch_ids() {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) id[q] = gg_sload(irs, (int)(iat + 32 * q), 0);
+    for (int u = 0; u < kSets; ++u)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) id[u][q] = gg_sload(irs, (int)(iat + 4 * WAVES * u + 32 * q), 0);
     iat += 256;
   }
-  // Row offset of the step whose ids were fetched (left: its reduction rows); fetches the next ids.
+  // Row offsets of the step whose ids were fetched (left: its reduction rows); fetches the next ids.
   __device__ __forceinline__ void take_ids(int left) {
-    int v = id[0];
 #pragma unroll
-    for (int q = 1; q < 8; ++q) v = rr == q ? id[q] : v;
-    rowoff = (uint32_t)v < rows && k < left ? (uint32_t)v * ld2 : kGgOob;
+    for (int u = 0; u < kSets; ++u) {
+      int v = id[u][0];
+#pragma unroll
+      for (int q = 1; q < 8; ++q) {
+        int t = id[u][q];
+        asm("" : "+s"(t));  // a select, not an indexed array in scratch memory
+        v = rr == q ? t : v;
+      }
+      rowoff[u] = (uint32_t)v < rows && k + WAVES * u < left ? (uint32_t)v * ld2 : kGgOob;
+    }
     fetch_ids();
   }
 
   __device__ __forceinline__ void first() {
-    const int64_t b = reinterpret_cast<int64_t>(base);
-    const int64_t n = bytes < 0 ? 0 : (bytes > kGgSpan ? kGgSpan : bytes);
-    rs = gg_u4{(uint32_t)b, (uint32_t)((uint64_t)b >> 32) & 0xffffu, (uint32_t)n, 0x00020000u};
+    rs = gg_desc(base, bytes);
     so = 0;
   }
   __device__ __forceinline__ void next() {
@@ -353,41 +404,42 @@ struct GgOperand {
       if (left < 64) tail(left);
     }
   }
-  // The LDS-DMA is opaque to the compiler: it would wait for every one in
-  // flight before any LDS read.  Arrival is waited for by count (arrived()).
   __device__ __forceinline__ void issue(uint32_t lds, int j) {
     uint32_t v = vo[j];
-    if constexpr (GATHER) v = __builtin_elementwise_add_sat(v, rowoff);  // kGgOob stays past the end
-    asm volatile("s_add_u32 m0, %0, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(v), "s"(rs),
-                 "s"(so), "i"(WAVES * j * 1024)
-                 : "m0", "scc");
+    if constexpr (GATHER) v = __builtin_elementwise_add_sat(v, rowoff[j % kSets]);  // kGgOob stays past the end
+    gg_dma(lds + WAVES * j * 1024, v, rs, so);
   }
 };
 
 // Fragments of 16 rows (columns when TR): lane (i, g) holds reduction elements
-// 32 h + 8 g .. + 7 of row i.  Lane part of the address; the rest is constant.
-template <bool TR>
+// 32 h + 8 g .. + 7 of row i.  A wave's x-th is the image's block X0 + SKIP x of
+// 16 rows (SKIP 1: X0 a multiple of 4; SKIP 2: X0 0 or 1).  Lane part of the
+// address here, the rest is constant.
+template <bool TR, int SKIP>
 struct GgReader {
-  uint32_t p[TR ? 4 : 2];
-  __device__ __forceinline__ void init(int wbase, int lane) {
+  static_assert(SKIP == 1 || SKIP == 2, "block maps");
+  uint32_t p[TR ? 4 / SKIP : 2];
+  __device__ __forceinline__ void init(int X0, int lane) {
     const int i = lane & 15, g = lane >> 4;
+    const int at = SKIP == 1 ? (X0 >> 2) * 8192 : 0, x0 = SKIP == 1 ? 0 : X0;
     if constexpr (!TR) {
-      const int pos = 64 * (wbase >> 6) + 8 * (i & 7) + ((wbase & 63) >> 3) + (i >> 3);
+      const int pos = 8 * (i & 7) + 2 * x0 + (i >> 3);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) p[h] = pos * 128 + 16 * ((4 * h + g) ^ gg_swz(pos));
+      for (int h = 0; h < 2; ++h) p[h] = at + pos * 128 + 16 * ((4 * h + g) ^ gg_swz(pos));
     } else {
       const int q = i >> 2, pp = i & 3, pos = 8 * q + g;  // + 4 h, + 32 for elements 4 .. 7
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        p[x] = (wbase >> 6) * 8192 + pos * 128 + 16 * ((2 * (((wbase & 63) >> 4) ^ x) + (pp >> 1)) ^ gg_swz_tr(pos)) + 8 * (pp & 1);
+      for (int x = 0; x < 4 / SKIP; ++x)
+        p[x] = at + pos * 128 + 16 * ((2 * (x0 + SKIP * x) + (pp >> 1)) ^ gg_swz_tr(pos)) + 8 * (pp & 1);
     }
   }
 };
 typedef __attribute__((address_space(3))) const gg_u4* gg_lu4;
-template <bool TR>
-__device__ __forceinline__ gg_u4 gg_frag(const GgReader<TR>& rd, uint32_t img, int h, int x) {
-  if constexpr (!TR) return *(gg_lu4)(uintptr_t)(rd.p[h] + img + (x >> 2) * 8192 + (x & 3) * 256);
-  const uint32_t a = rd.p[x & 3] + img + (x >> 2) * 8192 + h * 512;
+template <bool TR, int SKIP>
+__device__ __forceinline__ gg_u4 gg_frag(const GgReader<TR, SKIP>& rd, uint32_t img, int h, int x) {
+  constexpr int kIn = 4 / SKIP;  // blocks of one 64-row group (64-column image)
+  if constexpr (!TR) return *(gg_lu4)(uintptr_t)(rd.p[h] + img + (x / kIn) * 8192 + (x % kIn) * 256 * SKIP);
+  const uint32_t a = rd.p[x % kIn] + img + (x / kIn) * 8192 + h * 512;
   const gg_i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(uintptr_t)(a));
   const gg_i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gg_lv4)(uintptr_t)(a + 4096));
   const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
@@ -442,9 +494,17 @@ __device__ __forceinline__ void gg_order(int pos, int mt, int nt, int& mi, int& 
   ni += 8 * nb;
 }
 
+// Of all 256 x 256 tiles, how many run as such: whole rounds over the CUs, and a
+// last one only if it fills most of them.
+constexpr int kGgCus = 256, kGgFill = 112;
+__host__ __device__ __forceinline__ int gg_big(int all) {
+  const int last = all % kGgCus;
+  return last <= kGgFill ? all - last : all;
+}
+
 // BM x BN tile, WM x WN waves.
 template <int DT, int OP, int BM, int BN, int WM, int WN, bool GATHER>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(GroupedArgs a, int mt_max, int nt) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a, int big) {
   constexpr int W = WM * WN, XF = BM / WM / 16, YF = BN / WN / 16;
   constexpr bool TA = OP == kWgrad, TB = OP != kLinear;
   // units of 256 rows x 64: A of step t, B of step t, A of step t + 1, ...
@@ -462,31 +522,83 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   int64_t m0, red0 = 0;   // first output row; first reduction row (wgrad)
   int red;                // reduction length
   int n0;
+  // The grid in 256 x 256 tiles; the 128 x 128 kernel takes the last of them
+  // (big <= tile, four workgroups each) and the rows that fill no 256.
+  constexpr bool kSmall = BM == 128;
+  const int ntb = (cols + 255) / 256;
+  int sub_m = 0, sub_n = 0;  // kSmall: 128-row (column) half of the tile
   if constexpr (OP == kWgrad) {
-    const int per = mt_max * nt, pos = gg_pos(blockIdx.x, per * a.E);
-    if (pos < 0) return;
+    const int mtb = (a.N + 255) / 256, per = mtb * ntb;
+    int pos;
+    if constexpr (kSmall) {
+      pos = gg_pos(blockIdx.x, 4 * (per * a.E - big));
+      if (pos < 0) return;
+      sub_m = (pos >> 1) & 1;
+      sub_n = pos & 1;
+      pos = big + (pos >> 2);
+    } else {
+      pos = gg_pos(blockIdx.x, big);
+      if (pos < 0) return;
+    }
     e = pos / per;
     int mi, ni;
-    gg_order(pos - e * per, mt_max, nt, mi, ni);
-    m0 = (int64_t)mi * BM;
-    n0 = ni * BN;
+    gg_order(pos - e * per, mtb, ntb, mi, ni);
+    m0 = (int64_t)mi * 256 + 128 * sub_m;
+    n0 = ni * 256 + 128 * sub_n;
+    if (m0 >= a.N || n0 >= cols) return;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
     red0 = __builtin_amdgcn_readfirstlane((int)gg_clamp(a.offsets[e], 0, a.S));
     red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
   } else {
-    int ni = 0;
-    const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
-      const int pos = gg_pos(blockIdx.x, mts * nt);
-      if (pos < 0) return -1;
-      int mi;
-      gg_order(pos, mts, nt, mi, ni);
-      return mi;
-    });
-    if (t.e == -2) return;
-    n0 = ni * BN;
-    e = __builtin_amdgcn_readfirstlane(t.e);
-    m0 = __builtin_amdgcn_readfirstlane((int)t.s0);
-    mrows = __builtin_amdgcn_readfirstlane((int)(t.s1 - t.s0));
+    const GgGroups gr{a.offsets, a.E, a.S};
+    auto whole = [](int64_t rows) { return (int)(rows / 256); };
+    auto halves = [](int64_t rows) { return (int)((rows % 256 + 127) / 128); };
+    const int mtb = gr.total(whole), all = mtb * ntb, mine = gg_big(all);
+    int64_t lo, hi;
+    int mi, ni, in;
+    if constexpr (!kSmall) {
+      const int pos = gg_pos(blockIdx.x, mine);
+      if (pos < 0) return;
+      gg_order(pos, mtb, ntb, mi, ni);
+      if (!gr.find(mi, whole, e, lo, hi, in)) return;
+      m0 = lo + 256 * in;
+      mrows = 256;
+    } else {
+      const int nts = (cols + 127) / 128, mts = gr.total(halves);
+      int head = 0, tail = 0;
+      if (a.zero_rest) gr.rest(head, tail, 128);
+      int pos = gg_pos(blockIdx.x, 4 * (all - mine) + (mts + head + tail) * nts);
+      if (pos < 0) return;
+      if (pos < 4 * (all - mine)) {
+        gg_order(mine + (pos >> 2), mtb, ntb, mi, ni);
+        if (!gr.find(mi, whole, e, lo, hi, in)) return;
+        m0 = lo + 256 * in + 128 * ((pos >> 1) & 1);
+        mrows = 128;
+        n0 = 256 * ni + 128 * (pos & 1);
+        if (n0 >= cols) return;
+      } else {
+        pos -= 4 * (all - mine);  // strips of 8 row tiles
+        const int strip = pos / (8 * nts), r = pos - strip * 8 * nts, h = min(8, mts + head + tail - 8 * strip);
+        ni = r / h;
+        mi = 8 * strip + (r - ni * h);
+        n0 = 128 * ni;
+        if (mi < mts) {
+          if (!gr.find(mi, halves, e, lo, hi, in)) return;
+          m0 = lo + (hi - lo) / 256 * 256 + 128 * in;
+          mrows = (int)(hi - m0 < 128 ? hi - m0 : 128);
+        } else {
+          if (!gr.find_rest(mi - mts, 128, lo, hi)) return;
+          e = -1;
+          m0 = lo;
+          mrows = (int)(hi - lo);
+        }
+      }
+    }
+    if constexpr (!kSmall) n0 = ni * 256;
+    e = __builtin_amdgcn_readfirstlane(e);
+    m0 = __builtin_amdgcn_readfirstlane((int)m0);
+    n0 = __builtin_amdgcn_readfirstlane(n0);
+    mrows = __builtin_amdgcn_readfirstlane(mrows);
     red = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
   }
   const int ncols = cols - n0 < BN ? cols - n0 : BN;
@@ -559,7 +671,11 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   for (int x = 0; x < XF; ++x)
 #pragma unroll
     for (int y = 0; y < YF; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
-  const int wm = (w / WN) * (BM / WM), wn = (w % WN) * (BN / WN);
+  // wave (wr, wc): row blocks wr, wr + 2, ... of 16 (a tile that is not full keeps
+  // both wave rows busy, and blocks without rows are skipped), columns 64 wc ..
+  const int wr = w / WN, wc = w % WN, wn = wc * (BN / WN);
+  const bool sums = OP == kWgrad && a.db && n0 == 0;  // every wave column sums a part of dz
+  const int xn = wn < ncols || sums ? ((mrows + 15) / 16 - wr + 1) / 2 : 0;
 
   // A step has two halves of 32 deep.  A half's MFMAs run on fragments in
   // registers while the next half's are read from LDS and 32 KiB of a later step
@@ -572,13 +688,13 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   constexpr int kPA = GgOperand<BM, W, TA>::kPieces, kPB = GgOperand<BN, W, TB, GATHER>::kPieces;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
   asm volatile("" ::"v"(lds0) : "memory");
-  GgReader<TA> ra;
-  GgReader<TB> rb;
-  ra.init(wm, lane);
-  rb.init(wn, lane);
+  static_assert(WM == 2 && YF == 4, "block maps");
+  GgReader<TA, 2> ra;
+  GgReader<TB, 1> rb;
+  ra.init(wr, lane);
+  rb.init(YF * wc, lane);
   const uint32_t dma0 = lds0 + w * 1024;
   gg_u4 fa[2][XF], fb[2][YF];
-  const bool sums = OP == kWgrad && a.db && n0 == 0;
   constexpr uint32_t kOnes = DT == kBF16 ? 0x3f803f80u : 0x3c003c00u;
   const gg_u4 ones = {kOnes, kOnes, kOnes, kOnes};
   f32x4 accs[XF / WN > 0 ? XF / WN : 1];
@@ -596,9 +712,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     __builtin_amdgcn_sched_barrier(0);
   };
   // MFMAs on (ac, bc); read half h of images (ia, ib) into (an, bn)
-  auto half = [&](auto& op, uint32_t dst, int h, uint32_t ia, uint32_t ib, gg_u4 (&ac)[XF], gg_u4 (&bc)[YF], gg_u4 (&an)[XF],
+  auto half = [&](auto full, auto& op, uint32_t dst, int h, uint32_t ia, uint32_t ib, gg_u4 (&ac)[XF], gg_u4 (&bc)[YF], gg_u4 (&an)[XF],
                   gg_u4 (&bn)[YF], int left) {
-    constexpr int kR = XF + YF, kOver = XF - 2;
     if constexpr (GATHER) {  // before this half's LDS reads: the scalar loads share their counter
       if constexpr (std::is_same_v<std::decay_t<decltype(op)>, GgOperand<BN, W, TB, true>>) op.advance(left);
     }
@@ -608,23 +723,25 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
         if constexpr (!GATHER || !std::is_same_v<std::decay_t<decltype(op)>, GgOperand<BN, W, TB, true>>) op.advance(left);
       }
 #pragma unroll
-      for (int q = 0; q < kR; ++q)
-        if (q * kOver / kR == x) {
-          if (q < YF) bn[q] = gg_frag<TB>(rb, ib, h, q);
-          else an[q - YF] = gg_frag<TA>(ra, ia, h, q - YF);
-        }
-#pragma unroll
-      for (int j = 0; j < kPA; ++j)  // all after next()
+      for (int j = 0; j < kPA; ++j)  // all after advance()
         if (1 + j * (XF - 1) / kPA == x) op.issue(dst, j);
+      if (decltype(full)::value || x < xn) {
+        if (x == 0) {
 #pragma unroll
-      for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(bc[y], ac[x], acc[x][y]);
+          for (int y = 0; y < YF; ++y) bn[y] = gg_frag(rb, ib, h, y);
+          an[0] = gg_frag(ra, ia, h, 0);
+        }
+        if (x + 1 < XF) an[x + 1] = gg_frag(ra, ia, h, x + 1);
+#pragma unroll
+        for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(bc[y], ac[x], acc[x][y]);
+      }
       __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (OP == kWgrad) {
       if (sums) {  // column sums of dz: a product with ones, each wave of a row its part
 #pragma unroll
         for (int c = 0; c < WN; ++c)
-          if (w % WN == c) {
+          if (wc == c) {
 #pragma unroll
             for (int u = 0; u < XF / WN; ++u) accs[u] = gg_mfma<DT>(ones, ac[XF / WN * c + u], accs[u]);
           }
@@ -658,18 +775,22 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int y = 0; y < YF; ++y) fb[0][y] = gg_frag<TB>(rb, lds0 + kUnit, 0, y);
+    for (int y = 0; y < YF; ++y) fb[0][y] = gg_frag(rb, lds0 + kUnit, 0, y);
 #pragma unroll
-    for (int x = 0; x < XF; ++x) fa[0][x] = gg_frag<TA>(ra, lds0, 0, x);
-    uint32_t ua = 0;
-    for (int t = 0; t < steps; ++t) {
-      const int left = red - 64 * (t + 2);
-      const uint32_t ub = turn(ua + kUnit), va = turn(ua + 2 * kUnit), vb = turn(va + kUnit), fr = turn(vb + kUnit);
-      half(oa, dma0 + fr, 1, lds0 + ua, lds0 + ub, fa[0], fb[0], fa[1], fb[1], left);
-      sync();
-      half(ob, dma0 + ua, 0, lds0 + va, lds0 + vb, fa[1], fb[1], fa[0], fb[0], left);
-      ua = va;
-    }
+    for (int x = 0; x < XF; ++x) fa[0][x] = gg_frag(ra, lds0, 0, x);
+    auto run = [&](auto full) {
+      uint32_t ua = 0;
+      for (int t = 0; t < steps; ++t) {
+        const int left = red - 64 * (t + 2);
+        const uint32_t ub = turn(ua + kUnit), va = turn(ua + 2 * kUnit), vb = turn(va + kUnit), fr = turn(vb + kUnit);
+        half(full, oa, dma0 + fr, 1, lds0 + ua, lds0 + ub, fa[0], fb[0], fa[1], fb[1], left);
+        sync();
+        half(full, ob, dma0 + ua, 0, lds0 + va, lds0 + vb, fa[1], fb[1], fa[0], fb[0], left);
+        ua = va;
+      }
+    };
+    if (!kSmall || xn == XF) run(std::true_type{});
+    else run(std::false_type{});
     __builtin_amdgcn_s_waitcnt(0x0f70);  // no LDS-DMA outlives the workgroup
   }
 
@@ -680,13 +801,13 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     if (sums && g == 0) {
 #pragma unroll
       for (int u = 0; u < XF / WN; ++u) {
-        const int m = wm + 16 * (XF / WN * (w % WN) + u) + i;
+        const int m = 16 * (2 * (XF / WN * wc + u) + wr) + i;
         if (m < mrows) a.db[(int64_t)e * a.N + m0 + m] = accs[u][0];
       }
     }
 #pragma unroll
     for (int x = 0; x < XF; ++x) {
-      const int m = wm + 16 * x + i;
+      const int m = 16 * (2 * x + wr) + i;
       if (m >= mrows) continue;
       float* o = out + (m0 + m) * a.ldo + n0;
 #pragma unroll
@@ -723,7 +844,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
     const uint16_t* mk = OP == kDgrad && e >= 0 ? static_cast<const uint16_t*>(a.mask) : nullptr;
 #pragma unroll
     for (int x = 0; x < XF; ++x) {
-      const int m = wm + 16 * x + i;
+      const int m = 16 * (2 * x + wr) + i;
 #pragma unroll
       for (int y = 0; y < YF; y += 2) {
         // two neighbouring tiles: lanes of even g take the first, of odd g the
@@ -752,6 +873,175 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN / 4) void grouped_fast_k(Grou
   }
 }
 
+// ---------------------------------------------------------------------------
+// Few rows an expert (single tokens): the weights are read once and that is
+// the time.  A workgroup owns 64 output columns of up to 16 MX rows; its 4 waves
+// take the 64-deep steps in turn, each with a ring of its own (2 slots of 64
+// weight rows and 16 MX operand rows), so the loop has no barrier and 4 x 2 slots
+// a workgroup, two workgroups a CU, are in flight.  The waves' partial tiles are
+// summed in wave order through LDS.
+// ---------------------------------------------------------------------------
+template <int DT, int OP, int MX>
+__global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt) {
+  constexpr int BM = 16 * MX, BN = 64;
+  constexpr bool TB = OP == kDgrad;
+  constexpr int kW = 8192, kX = BM * 128, kStage = kW + kX, kPX = BM / 8;  // bytes and pieces of a stage
+  __shared__ __attribute__((aligned(1024))) char lds[4 * 2 * kStage];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int rr = lane >> 3, p = lane & 7, i = lane & 15, g = lane >> 4;
+  const int cols = OP == kLinear ? a.N : a.K;
+  // an XCD takes every 8th column tile, all its row tiles together
+  int ni = 0;
+  const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
+    if (mts == 0) return -1;
+    const int j = blockIdx.x >> 3;
+    ni = (blockIdx.x & 7) + 8 * (j / mts);
+    return ni < nt ? j % mts : -1;
+  });
+  if (t.e == -2) return;
+  const int e = __builtin_amdgcn_readfirstlane(t.e);
+  const int64_t m0 = __builtin_amdgcn_readfirstlane((int)t.s0);
+  const int mrows = __builtin_amdgcn_readfirstlane((int)(t.s1 - t.s0));
+  const int red = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
+  const int n0 = ni * BN, ncols = cols - n0 < BN ? cols - n0 : BN;
+
+  // weights: as one operand of 64 rows (columns)
+  GgOperand<64, 1, TB> ob;
+  const char* B = static_cast<const char*>(a.b);
+  if constexpr (!TB) {
+    ob.c8 = 8 * p;
+    ob.base = gg_uni(B + ((int64_t)e * a.strb + (int64_t)n0 * a.ldb) * 2);
+    ob.bytes = gg_uni(((int64_t)(ncols - 1) * a.ldb + red) * 2);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = j + 8 * rr;
+      ob.vo[j] = r < ncols ? (uint32_t)((r * a.ldb + (ob.c8 ^ (8 * j))) * 2) : kGgOob;
+    }
+  } else {
+    ob.base = gg_uni(B + ((int64_t)e * a.strb + n0) * 2);
+    ob.bytes = gg_uni(((int64_t)(red - 1) * a.ldb + ncols) * 2);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = j + 8 * rr, c = 8 * (p ^ gg_swz_tr(8 * j + rr));
+      ob.vo[j] = c < ncols ? (uint32_t)((r * a.ldb + c) * 2) : kGgOob;
+    }
+  }
+  // operand rows in their order, chunk c of row r at c ^ ((r >> 1) & 7)
+  const bool gather = OP == kLinear && a.rows;
+  const char* A = static_cast<const char*>(a.a);
+  const gg_u4 ars = gg_desc(gg_uni(gather ? A : A + m0 * a.lda * 2),
+                            gg_uni(gather ? ((a.T - 1) * a.lda + red) * 2 : ((int64_t)(mrows - 1) * a.lda + red) * 2));
+  uint32_t av[kPX];
+  int ac[kPX];
+#pragma unroll
+  for (int j = 0; j < kPX; ++j) {
+    const int r = 8 * j + rr;
+    ac[j] = 8 * (p ^ ((r >> 1) & 7));
+    int64_t row = r;
+    bool ok = r < mrows && e >= 0;
+    if (gather) {
+      row = ok ? a.rows[m0 + r] : 0;
+      ok = ok && row >= 0 && row < a.T;
+    }
+    av[j] = ok ? (uint32_t)((row * a.lda + ac[j]) * 2) : kGgOob;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
+  asm volatile("" ::"v"(lds0) : "memory");
+  const uint32_t ring = lds0 + w * 2 * kStage;
+  const int steps = (red + 63) / 64;
+  const int mine = steps > w ? (steps - w + 3) / 4 : 0;  // steps w, w + 4, ...
+  auto stage = [&](int j, uint32_t at) {
+    const int st = w + 4 * j, left = red - 64 * st;
+    const uint32_t so = (uint32_t)st * 128u;
+    gg_u4 rs;
+    if constexpr (!TB) rs = gg_desc(ob.base, ob.bytes);
+    else rs = gg_desc(ob.base + (int64_t)st * 64 * a.ldb * 2, ob.bytes - (int64_t)st * 64 * a.ldb * 2);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      uint32_t v = ob.vo[q];
+      if constexpr (!TB) v = (ob.c8 ^ (8 * q)) < left ? v : kGgOob;
+      gg_dma(at + 1024 * q, v, rs, TB ? 0u : so);
+    }
+#pragma unroll
+    for (int q = 0; q < kPX; ++q) gg_dma(at + kW + 1024 * q, ac[q] < left ? av[q] : kGgOob, ars, so);
+  };
+  GgReader<TB, 1> rb;
+  rb.init(0, lane);
+  uint32_t rx[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) rx[h] = i * 128 + 16 * ((4 * h + g) ^ ((i >> 1) & 7));
+  f32x4 acc[MX][4];
+#pragma unroll
+  for (int x = 0; x < MX; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
+  if (mine > 0) stage(0, ring);
+  if (mine > 1) stage(1, ring + kStage);
+  for (int j = 0; j < mine; ++j) {
+    asm volatile("" ::: "memory");
+    if (j + 1 < mine) gg_wait<8 + kPX>();
+    else gg_wait<0>();
+    asm volatile("" ::: "memory");
+    const uint32_t at = ring + (j & 1) * kStage;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      gg_u4 fa[MX], fb[4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y) fb[y] = gg_frag(rb, at, h, y);
+#pragma unroll
+      for (int x = 0; x < MX; ++x) fa[x] = *(gg_lu4)(uintptr_t)(at + kW + rx[h] + x * 2048);
+#pragma unroll
+      for (int x = 0; x < MX; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) acc[x][y] = gg_mfma<DT>(fb[y], fa[x], acc[x][y]);
+    }
+    asm volatile("" ::: "memory");
+    if (j + 2 < mine) {
+      gg_wait<8 + kPX>();  // this slot has been read
+      asm volatile("" ::: "memory");
+      stage(j + 2, at);
+    }
+  }
+  __syncthreads();  // every wave is out of its ring
+  constexpr int kPitch = 68;
+  float* red_t = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int x = 0; x < MX; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      *reinterpret_cast<f32x4*>(red_t + (w * BM + 16 * x + i) * kPitch + 16 * y + 4 * g) = acc[x][y];
+  __syncthreads();
+  const int c = 4 * (tid & 15), n = n0 + c;
+#pragma unroll
+  for (int x = 0; x < MX; ++x) {
+    const int m = 16 * x + (tid >> 4);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v += *reinterpret_cast<const f32x4*>(red_t + (q * BM + m) * kPitch + c);
+    if (m >= mrows || c >= ncols) continue;
+    if constexpr (OP == kLinear) {
+      if (e >= 0 && a.bias) {
+        const float* bp = a.bias + (int64_t)e * a.ldbias + n;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] += bp[q];
+      }
+      if (a.relu) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
+      }
+    } else {
+      if (e >= 0 && a.mask) {
+        const uint2 k = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(a.mask) + (m0 + m) * a.ldmask + n);
+        const uint16_t mk[4] = {(uint16_t)k.x, (uint16_t)(k.x >> 16), (uint16_t)k.y, (uint16_t)(k.y >> 16)};
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = gg_f<DT>(mk[q]) > 0.f ? v[q] : 0.f;
+      }
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (m0 + m) * a.ldo + n) =
+        make_uint2(gg_pack2<DT>(v[0], v[1]), gg_pack2<DT>(v[2], v[3]));
+  }
+}
+
 bool gg_al(const void* p, int64_t ld, int64_t need) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld >= need;
 }
@@ -770,30 +1060,66 @@ bool fast_ok(GroupedOp op, const GroupedArgs& a) {
   return op != kDgrad || !a.mask || gg_al(a.mask, a.ldmask, 0);
 }
 
-template <int DT, int OP, int BM, int BN, int WM, int WN, bool GATHER = false>
+template <int DT, int OP, bool GATHER = false>
 hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
   const int cols = OP == kLinear ? a.N : a.K;
-  const int nt = (cols + BN - 1) / BN;
-  int64_t mt;
-  if (OP == kWgrad) mt = (a.N + BM - 1) / BM;
-  else {
-    mt = (a.S + BM - 1) / BM + a.E + (a.zero_rest ? 2 : 0);
-    mt = mt < a.S ? mt : a.S;
+  const int64_t ntb = (cols + 255) / 256, nts = (cols + 127) / 128;
+  int64_t big, small;  // workgroups at most
+  int keep = 0;
+  if (OP == kWgrad) {
+    const int64_t all = (a.N + 255) / 256 * ntb * a.E;
+    if (all > 0x3fffffffLL) return hipErrorInvalidValue;
+    keep = gg_big((int)all);
+    big = keep;
+    small = 4 * (all - keep);
+  } else {
+    const int64_t all = a.S / 256 * ntb;
+    big = all > kGgFill ? all : 0;  // fewer never run as 256 x 256
+    small = 4 * (all < kGgFill ? all : kGgFill) + ((int64_t)a.E * 2 + (a.zero_rest ? a.S / 128 + 2 : 0)) * nts;
+    const int64_t most = (a.S + 127) / 128 + a.E + (a.zero_rest ? 2 : 0);
+    small = small < most * nts ? small : most * nts;
+    if (a.S < 128 * most) small = small < a.S * nts ? small : a.S * nts;
   }
-  const int64_t tiles = mt * nt * (OP == kWgrad ? a.E : 1), blocks = (tiles + 7) / 8 * 8;  // the XCDs in turn
+  big = (big + 7) / 8 * 8;
+  small = (small + 7) / 8 * 8;
+  if (big > 0x7fffff00LL || small > 0x7fffff00LL) return hipErrorInvalidValue;
+  if (big)
+    hipLaunchKernelGGL((grouped_fast_k<DT, OP, 256, 256, 2, 4, GATHER>), dim3((uint32_t)big), dim3(512), 0, s, a, keep);
+  if (small)
+    hipLaunchKernelGGL((grouped_fast_k<DT, OP, 128, 128, 2, 2, GATHER>), dim3((uint32_t)small), dim3(256), 0, s, a, keep);
+  return hipGetLastError();
+}
+
+template <int DT, int OP, int MX>
+hipError_t launch_skinny(const GroupedArgs& a, hipStream_t s) {
+  const int cols = OP == kLinear ? a.N : a.K;
+  const int nt = (cols + 63) / 64;
+  int64_t mt = (a.S + 16 * MX - 1) / (16 * MX) + a.E + (a.zero_rest ? 2 : 0);
+  mt = mt < a.S ? mt : a.S;
+  const int64_t blocks = (int64_t)(nt + 7) / 8 * 8 * mt;
   if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((grouped_fast_k<DT, OP, BM, BN, WM, WN, GATHER>), dim3((uint32_t)blocks), dim3(64 * WM * WN), 0, s, a,
-                     (int)mt, nt);
+  hipLaunchKernelGGL((grouped_skinny_k<DT, OP, MX>), dim3((uint32_t)blocks), dim3(256), 0, s, a, nt);
   return hipGetLastError();
 }
 template <int DT>
-hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
-  switch (op) {
-    case kLinear: return launch_fast<DT, kLinear, 256, 256, 2, 4>(a, s);
-    case kDgrad: return launch_fast<DT, kDgrad, 256, 256, 2, 4>(a, s);
-    default:
-      return a.rows ? launch_fast<DT, kWgrad, 256, 256, 2, 4, true>(a, s) : launch_fast<DT, kWgrad, 256, 256, 2, 4>(a, s);
+hipError_t launch_skinny_op(GroupedOp op, const GroupedArgs& a, int mx, hipStream_t s) {
+  if (op == kLinear) {
+    if (mx == 1) return launch_skinny<DT, kLinear, 1>(a, s);
+    return launch_skinny<DT, kLinear, 2>(a, s);
   }
+  if (mx == 1) return launch_skinny<DT, kDgrad, 1>(a, s);
+  return launch_skinny<DT, kDgrad, 2>(a, s);
+}
+
+template <int DT>
+hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
+  if (op == kWgrad) return a.rows ? launch_fast<DT, kWgrad, true>(a, s) : launch_fast<DT, kWgrad>(a, s);
+  // single tokens: by the mean rows of an expert
+  const int64_t mean = a.S / a.E;
+  const int red = op == kLinear ? a.K : a.N;
+  if (mean <= 16) return launch_skinny_op<DT>(op, a, 1, s);
+  if (mean <= 32 && red >= 2048) return launch_skinny_op<DT>(op, a, 2, s);
+  return op == kLinear ? launch_fast<DT, kLinear>(a, s) : launch_fast<DT, kDgrad>(a, s);
 }
 
 }  // namespace
