@@ -75,20 +75,24 @@ struct GgGroups {
   const int32_t* off;
   int E;
   int64_t S;
+  int a0, b0;  // the first 64 groups', in the lanes
 
-  __device__ __forceinline__ void bounds(int e, int64_t& a, int64_t& b) const {
-    a = gg_clamp(off[e], 0, S);
-    b = gg_clamp(off[e + 1], a, S);
+  __device__ __forceinline__ GgGroups(const int32_t* o, int e, int64_t s) : off(o), E(e), S(s) { bounds(0, a0, b0); }
+  __device__ __forceinline__ void bounds(int e0, int& a, int& b) const {
+    const int e = e0 + (threadIdx.x & 63);
+    a = b = 0;
+    if (e < E) {
+      a = (int)gg_clamp(off[e], 0, S);
+      b = (int)gg_clamp(off[e + 1], a, S);
+    }
   }
   template <class Count>
   __device__ __forceinline__ void scan(int e0, Count count, int& a, int& b, int& n, int& inc) const {
-    const int lane = threadIdx.x & 63;
-    a = b = 0;
-    if (e0 + lane < E) {
-      int64_t x, y;
-      bounds(e0 + lane, x, y);
-      a = (int)x;
-      b = (int)y;
+    if (e0 == 0) {
+      a = a0;
+      b = b0;
+    } else {
+      bounds(e0, a, b);
     }
     n = count((int64_t)b - a);
     inc = gg_scan64(n);
@@ -141,7 +145,7 @@ struct GgGroups {
 // (zero_rest) those of the rows in no group.
 template <class Pick>
 __device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, int BM, bool zero_rest, Pick pick) {
-  const GgGroups gr{off, E, S};
+  const GgGroups gr(off, E, S);
   auto count = [BM](int64_t rows) { return (int)((rows + BM - 1) / BM); };
   const int total = gr.total(count);
   int head = 0, tail = 0;
@@ -494,12 +498,62 @@ __device__ __forceinline__ void gg_order(int pos, int mt, int nt, int& mi, int& 
   ni += 8 * nb;
 }
 
-// Of all 256 x 256 tiles, how many run as such: whole rounds over the CUs, and a
-// last one only if it fills most of them.
-constexpr int kGgCus = 256, kGgFill = 112;
-__host__ __device__ __forceinline__ int gg_big(int all) {
-  const int last = all % kGgCus;
-  return last <= kGgFill ? all - last : all;
+// Which tiles run as 256 x 256 and which as 128 x 128, from what is known on the
+// GPU only: both kernels make the same choice.  A round of 256 x 256 tiles over
+// the CUs takes as long as about 540 tiles of 128 x 128 (which move twice the
+// bytes a product: 1250 against 700 TFLOP/s), and a launch of few of those as long
+// as 190; a round that is not full costs a whole one.  So the last round, and the
+// groups' last rows that fill no 256, go where they are done sooner.
+constexpr int kGgCus = 256, kGgRound = 540, kGgSmallMin = 190, kGgGap = 1300;
+// (a second launch costs about 4 us: kGgGap tiles at one step each)
+__host__ __device__ __forceinline__ int64_t gg_small_cost(int64_t tiles, int steps) {
+  return tiles == 0 ? 0 : (tiles > kGgSmallMin ? tiles : kGgSmallMin) + kGgGap / (steps > 0 ? steps : 1);
+}
+struct GgPlan {
+  int whole, mt;   // row tiles of 256: full ones, all of this plan (the others have fewer rows)
+  int big;         // tiles of the mt x ntb grid run as 256 x 256, in gg_order; the rest in quarters
+  int halves;      // 128-row tiles of the rows that fill no 256, when the plan leaves those out
+};
+__device__ __forceinline__ GgPlan gg_plan(const GgGroups& gr, int ntb, int nts, int steps, bool only_small) {
+  const int f = gr.total([](int64_t r) { return (int)(r / 256); });
+  const int p = gr.total([](int64_t r) { return r % 256 ? 1 : 0; });
+  const int h = gr.total([](int64_t r) { return (int)((r % 256 + 127) / 128); });
+  GgPlan best{f, f, 0, h};
+  if (only_small) return best;
+  int64_t least = -1;
+#pragma unroll
+  for (int o = 0; o < 4; ++o) {
+    const bool part = o & 1, up = !(o & 2);
+    const int mt = part ? f + p : f;
+    const int64_t q = (int64_t)mt * ntb, last = q % kGgCus, whole = q - last;
+    const int64_t extra = part ? 0 : (int64_t)h * nts;
+    const int64_t lp = part ? (last < (int64_t)p * ntb ? last : (int64_t)p * ntb) : 0;  // not full: these come last
+    const int64_t tail = 4 * (last - lp) + (lp ? 2 * lp * h / p : 0);
+    const int64_t cost = up ? (q + kGgCus - 1) / kGgCus * kGgRound + gg_small_cost(extra, steps)
+                            : q / kGgCus * kGgRound + gg_small_cost(tail + extra, steps);
+    if (least < 0 || cost < least) {
+      least = cost;
+      best.mt = mt;
+      best.big = (int)(up ? q : whole);
+      best.halves = part ? 0 : h;
+    }
+  }
+  return best;
+}
+// Rows of row tile mi of a plan's grid.
+__device__ __forceinline__ bool gg_rows(const GgGroups& gr, const GgPlan& pl, int mi, int& e, int64_t& m0, int& rows) {
+  int64_t lo, hi;
+  int in;
+  if (mi < pl.whole) {
+    if (!gr.find(mi, [](int64_t r) { return (int)(r / 256); }, e, lo, hi, in)) return false;
+    m0 = lo + 256 * in;
+    rows = 256;
+  } else {
+    if (!gr.find(mi - pl.whole, [](int64_t r) { return r % 256 ? 1 : 0; }, e, lo, hi, in)) return false;
+    rows = (int)((hi - lo) % 256);
+    m0 = hi - rows;
+  }
+  return true;
 }
 
 // BM x BN tile, WM x WN waves.
@@ -550,51 +604,50 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
     red0 = __builtin_amdgcn_readfirstlane((int)gg_clamp(a.offsets[e], 0, a.S));
     red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
   } else {
-    const GgGroups gr{a.offsets, a.E, a.S};
-    auto whole = [](int64_t rows) { return (int)(rows / 256); };
-    auto halves = [](int64_t rows) { return (int)((rows % 256 + 127) / 128); };
-    const int mtb = gr.total(whole), all = mtb * ntb, mine = gg_big(all);
-    int64_t lo, hi;
-    int mi, ni, in;
+    const GgGroups gr(a.offsets, a.E, a.S);
+    const int nts = (cols + 127) / 128;
+    const GgPlan pl = gg_plan(gr, ntb, nts, ((OP == kLinear ? a.K : a.N) + 63) / 64, big < 0);
+    int mi, ni;
     if constexpr (!kSmall) {
-      const int pos = gg_pos(blockIdx.x, mine);
+      const int pos = gg_pos(blockIdx.x, pl.big);
       if (pos < 0) return;
-      gg_order(pos, mtb, ntb, mi, ni);
-      if (!gr.find(mi, whole, e, lo, hi, in)) return;
-      m0 = lo + 256 * in;
-      mrows = 256;
+      gg_order(pos, pl.mt, ntb, mi, ni);
+      if (!gg_rows(gr, pl, mi, e, m0, mrows)) return;
+      n0 = ni * 256;
     } else {
-      const int nts = (cols + 127) / 128, mts = gr.total(halves);
       int head = 0, tail = 0;
       if (a.zero_rest) gr.rest(head, tail, 128);
-      int pos = gg_pos(blockIdx.x, 4 * (all - mine) + (mts + head + tail) * nts);
+      const int quarters = 4 * (pl.mt * ntb - pl.big), mts = pl.halves + head + tail;
+      int pos = gg_pos(blockIdx.x, quarters + mts * nts);
       if (pos < 0) return;
-      if (pos < 4 * (all - mine)) {
-        gg_order(mine + (pos >> 2), mtb, ntb, mi, ni);
-        if (!gr.find(mi, whole, e, lo, hi, in)) return;
-        m0 = lo + 256 * in + 128 * ((pos >> 1) & 1);
-        mrows = 128;
+      if (pos < quarters) {
+        gg_order(pl.big + (pos >> 2), pl.mt, ntb, mi, ni);
+        if (!gg_rows(gr, pl, mi, e, m0, mrows)) return;
+        const int sub = 128 * ((pos >> 1) & 1);
+        m0 += sub;
+        mrows = mrows - sub < 128 ? mrows - sub : 128;
         n0 = 256 * ni + 128 * (pos & 1);
-        if (n0 >= cols) return;
+        if (mrows <= 0 || n0 >= cols) return;
       } else {
-        pos -= 4 * (all - mine);  // strips of 8 row tiles
-        const int strip = pos / (8 * nts), r = pos - strip * 8 * nts, h = min(8, mts + head + tail - 8 * strip);
+        pos -= quarters;  // strips of 8 row tiles
+        const int strip = pos / (8 * nts), r = pos - strip * 8 * nts, h = mts - 8 * strip < 8 ? mts - 8 * strip : 8;
         ni = r / h;
         mi = 8 * strip + (r - ni * h);
         n0 = 128 * ni;
-        if (mi < mts) {
-          if (!gr.find(mi, halves, e, lo, hi, in)) return;
+        int64_t lo, hi;
+        int in;
+        if (mi < pl.halves) {
+          if (!gr.find(mi, [](int64_t x) { return (int)((x % 256 + 127) / 128); }, e, lo, hi, in)) return;
           m0 = lo + (hi - lo) / 256 * 256 + 128 * in;
           mrows = (int)(hi - m0 < 128 ? hi - m0 : 128);
         } else {
-          if (!gr.find_rest(mi - mts, 128, lo, hi)) return;
+          if (!gr.find_rest(mi - pl.halves, 128, lo, hi)) return;
           e = -1;
           m0 = lo;
           mrows = (int)(hi - lo);
         }
       }
     }
-    if constexpr (!kSmall) n0 = ni * 256;
     e = __builtin_amdgcn_readfirstlane(e);
     m0 = __builtin_amdgcn_readfirstlane((int)m0);
     n0 = __builtin_amdgcn_readfirstlane(n0);
@@ -1069,16 +1122,20 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
   if (OP == kWgrad) {
     const int64_t all = (a.N + 255) / 256 * ntb * a.E;
     if (all > 0x3fffffffLL) return hipErrorInvalidValue;
-    keep = gg_big((int)all);
+    const int64_t last = all % kGgCus;  // a last round in quarters where that is sooner
+    keep = (int)(gg_small_cost(4 * last, (int)(a.S / a.E / 64)) < kGgRound ? all - last : all);
     big = keep;
     small = 4 * (all - keep);
   } else {
-    const int64_t all = a.S / 256 * ntb;
-    big = all > kGgFill ? all : 0;  // fewer never run as 256 x 256
-    small = 4 * (all < kGgFill ? all : kGgFill) + ((int64_t)a.E * 2 + (a.zero_rest ? a.S / 128 + 2 : 0)) * nts;
-    const int64_t most = (a.S + 127) / 128 + a.E + (a.zero_rest ? 2 : 0);
-    small = small < most * nts ? small : most * nts;
-    if (a.S < 128 * most) small = small < a.S * nts ? small : a.S * nts;
+    // too few tiles for a round of 256 x 256, if half the groups end inside one
+    const int64_t some = a.E < a.S ? a.E : a.S;
+    if (4 * (a.S / 256 + some / 2) * ntb <= kGgRound) keep = -1;
+    big = keep < 0 ? 0 : (a.S / 256 + some) * ntb;
+    // quarters, halves of the groups' last rows, rows in no group
+    const int64_t quarters = keep < 0 ? a.S / 256 * ntb : kGgCus;
+    small = 4 * quarters + 2 * some * nts + (a.zero_rest ? (a.S / 128 + 2) * nts : 0);
+    const int64_t most = (a.S / 128 + 2 * some + 2) * 2 * ntb;
+    small = small < most ? small : most;
   }
   big = (big + 7) / 8 * 8;
   small = (small + 7) / 8 * 8;
