@@ -166,135 +166,6 @@ __device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, 
 }
 
 // ---------------------------------------------------------------------------
-// Any size, stride and alignment: 64 x 64 output tile, 4 waves of 32 x 32,
-// operands loaded element by element into LDS as [row][reduction].
-// ---------------------------------------------------------------------------
-constexpr int kGgBk = 32;
-constexpr int kGgPitch = 40;  // elements of an LDS row (80 B: 16-B aligned fragments)
-
-template <int DT, int OP>
-__global__ __launch_bounds__(256) void grouped_any_k(GroupedArgs a) {
-  __shared__ __attribute__((aligned(16))) uint16_t la[64 * kGgPitch], lb[64 * kGgPitch];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const uint16_t* A = static_cast<const uint16_t*>(a.a);
-  const uint16_t* B = static_cast<const uint16_t*>(a.b);
-  int e, n0 = 64 * blockIdx.y;
-  int64_t m0, m1, r0, r1;  // output rows [m0, m1), reduction [r0, r1)
-  const int ncols = OP == kLinear ? a.N : a.K;
-  if constexpr (OP == kWgrad) {
-    e = blockIdx.z;
-    m0 = 64 * (int64_t)blockIdx.x;
-    m1 = m0 + 64 < a.N ? m0 + 64 : a.N;
-    r0 = gg_clamp(a.offsets[e], 0, a.S);
-    r1 = gg_clamp(a.offsets[e + 1], r0, a.S);
-  } else {
-    const GgTile t = gg_find(a.offsets, a.E, a.S, 64, a.zero_rest, [](int) { return (int)blockIdx.x; });
-    if (t.e == -2) return;
-    e = t.e; m0 = t.s0; m1 = t.s1;
-    r0 = 0;
-    r1 = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
-  }
-  f32x4 acc[2][2];
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
-  float dbias = 0.f;
-  const int wm = 32 * (w >> 1), wn = 32 * (w & 1), i = lane & 15, g = lane >> 4;
-  for (int64_t r = r0; r < r1; r += kGgBk) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      // consecutive threads walk the operand's contiguous axis
-      uint16_t va = 0, vb = 0;
-      int ra, ka, rb, kb;
-      if constexpr (OP == kWgrad) {
-        ra = tid & 63; ka = (tid >> 6) + 4 * q;
-        rb = ra; kb = ka;
-        const int64_t s = r + ka;
-        if (s < r1) {
-          if (m0 + ra < m1) va = A[s * a.lda + m0 + ra];
-          const int64_t row = a.rows ? a.rows[s] : s;
-          if (row >= 0 && row < a.T && n0 + rb < ncols) vb = B[row * a.ldb + n0 + rb];
-        }
-      } else {
-        ka = tid & 31; ra = (tid >> 5) + 8 * q;
-        const int64_t s = m0 + ra;
-        if (s < m1 && r + ka < r1) {
-          const int64_t row = OP == kLinear && a.rows ? a.rows[s] : s;
-          if (OP != kLinear || (row >= 0 && row < a.T)) va = A[row * a.lda + r + ka];
-        }
-        if constexpr (OP == kLinear) {
-          kb = ka; rb = ra;
-          if (n0 + rb < ncols && r + kb < r1) vb = B[e * a.strb + (int64_t)(n0 + rb) * a.ldb + r + kb];
-        } else {
-          rb = tid & 63; kb = (tid >> 6) + 4 * q;
-          if (n0 + rb < ncols && r + kb < r1) vb = B[e * a.strb + (r + kb) * a.ldb + n0 + rb];
-        }
-      }
-      la[ra * kGgPitch + ka] = va;
-      lb[rb * kGgPitch + kb] = vb;
-    }
-    __syncthreads();
-    uint4 fa[2], fb[2];
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      fa[x] = *reinterpret_cast<const uint4*>(la + (wm + 16 * x + i) * kGgPitch + 8 * g);
-      fb[x] = *reinterpret_cast<const uint4*>(lb + (wn + 16 * x + i) * kGgPitch + 8 * g);
-    }
-#pragma unroll
-    for (int x = 0; x < 2; ++x)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) acc[x][y] = gg_mfma16<DT>(fa[x], fb[y], acc[x][y]);
-    if constexpr (OP == kWgrad) {
-      if (a.db && blockIdx.y == 0 && tid < 64)
-        for (int k = 0; k < kGgBk; ++k) dbias += gg_f<DT>(la[tid * kGgPitch + k]);
-    }
-    __syncthreads();
-  }
-  if constexpr (OP == kWgrad) {
-    if (a.db && blockIdx.y == 0 && tid < 64 && m0 + tid < m1) a.db[(int64_t)e * a.N + m0 + tid] = dbias;
-  }
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int y = 0; y < 2; ++y) {
-      const int n = n0 + wn + 16 * y + i;
-      if (n >= ncols) continue;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t m = m0 + wm + 16 * x + 4 * g + q;
-        if (m >= m1) continue;
-        float v = acc[x][y][q];
-        if constexpr (OP == kLinear) {
-          if (e >= 0) {
-            if (a.bias) v += a.bias[(int64_t)e * a.ldbias + n];
-            if (a.relu) v = v < 0.f ? 0.f : v;  // NaN stays NaN
-          }
-        } else if constexpr (OP == kDgrad) {
-          if (e >= 0 && a.mask && !(gg_f<DT>(static_cast<const uint16_t*>(a.mask)[m * a.ldmask + n]) > 0.f)) v = 0.f;
-        }
-        if constexpr (OP == kWgrad) static_cast<float*>(a.out)[e * a.stro + m * a.ldo + n] = v;
-        else static_cast<uint16_t*>(a.out)[m * a.ldo + n] = gg_h<DT>(v);
-      }
-    }
-}
-
-template <int DT>
-hipError_t launch_any(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
-  const int64_t tiles = (a.S + 63) / 64 + a.E + (a.zero_rest ? 2 : 0);
-  if (op == kWgrad) {
-    const dim3 grid((a.N + 63) / 64, (a.K + 63) / 64, a.E);
-    hipLaunchKernelGGL((grouped_any_k<DT, kWgrad>), grid, dim3(256), 0, s, a);
-  } else {
-    const int cols = op == kLinear ? a.N : a.K;
-    const dim3 grid((uint32_t)(tiles < a.S ? tiles : a.S), (cols + 63) / 64);
-    if (op == kLinear) hipLaunchKernelGGL((grouped_any_k<DT, kLinear>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((grouped_any_k<DT, kDgrad>), grid, dim3(256), 0, s, a);
-  }
-  return hipGetLastError();
-}
-
-// ---------------------------------------------------------------------------
 // Fast path: widths and row strides of whole 16-B words.  256 x 256 output
 // tile, 64-deep steps, 8 waves of 128 x 64 (16x16x32 MFMA), operands by LDS-DMA
 // into two buffers.
@@ -1093,6 +964,254 @@ __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt
     *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + (m0 + m) * a.ldo + n) =
         make_uint2(gg_pack2<DT>(v[0], v[1]), gg_pack2<DT>(v[2], v[3]));
   }
+}
+
+// ---------------------------------------------------------------------------
+// Any width, stride and alignment (rows of odd length start at any 2 bytes, so
+// nothing can go straight to LDS): 128 x 128 tile, 4 waves of 64 x 64, the same
+// LDS images; a thread loads 16-B chunks of a step into registers while the
+// step before is multiplied, and stores them into the other buffer after.
+// ---------------------------------------------------------------------------
+// 8 elements from column c of a row that has `limit` of them; 0 behind it.
+__device__ __forceinline__ gg_u4 gg_load8(const uint16_t* row, int c, int limit) {
+  if (c + 8 <= limit) {
+    gg_u4 v;
+    __builtin_memcpy(&v, row + c, 16);
+    return v;
+  }
+  uint64_t lo = 0, hi = 0;
+  if (limit >= 8) {  // the row's last 8, shifted
+    uint64_t v[2];
+    __builtin_memcpy(v, row + (limit - 8), 16);
+    const int sh = c - (limit - 8);
+    if (sh < 4) {
+      lo = (v[0] >> (16 * sh)) | (v[1] << (63 - 16 * sh) << 1);  // sh > 0: the chunk does not fit
+      hi = v[1] >> (16 * sh);
+    } else if (sh < 8) {
+      lo = v[1] >> (16 * (sh - 4));
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+      if (c + i < limit) (i < 4 ? lo : hi) |= (uint64_t)row[c + i] << (16 * (i & 3));
+  }
+  return gg_u4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
+template <int DT, int OP>
+__global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
+  constexpr int BM = 128, BN = 128, XF = 4, YF = 4;
+  constexpr bool TA = OP == kWgrad, TB = OP != kLinear;
+  constexpr uint32_t kImg = BM * 128;
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kImg];  // A, B, and again
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4, wr = w >> 1, wc = w & 1, wn = 64 * wc;
+  const int cols = OP == kLinear ? a.N : a.K, nt = (cols + BN - 1) / BN;
+  const uint16_t* A = static_cast<const uint16_t*>(a.a);
+  const uint16_t* B = static_cast<const uint16_t*>(a.b);
+  int e, mrows, red, ni = 0;
+  int64_t m0, red0 = 0;
+  if constexpr (OP == kWgrad) {
+    const int mtb = (a.N + BM - 1) / BM, per = mtb * nt, pos = gg_pos(blockIdx.x, per * a.E);
+    if (pos < 0) return;
+    e = pos / per;
+    int mi;
+    gg_order(pos - e * per, mtb, nt, mi, ni);
+    m0 = (int64_t)mi * BM;
+    mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
+    red0 = gg_clamp(a.offsets[e], 0, a.S);
+    red = (int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0);
+  } else {
+    const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
+      const int pos = gg_pos(blockIdx.x, mts * nt);
+      if (pos < 0) return -1;
+      int mi;
+      gg_order(pos, mts, nt, mi, ni);
+      return mi;
+    });
+    if (t.e == -2) return;
+    e = t.e;
+    m0 = t.s0;
+    mrows = (int)(t.s1 - t.s0);
+    red = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
+  }
+  const int n0 = ni * BN, ncols = cols - n0 < BN ? cols - n0 : BN;
+
+  // chunk q = tid + 256 j of a step: row-major operands row q / 8, chunk q % 8;
+  // transposed ones reduction row q / 16, column chunk q % 16
+  int64_t arow[4];  // this thread's rows of a row-major A, -1: none
+  if constexpr (!TA) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = (tid >> 3) + 32 * j;
+      arow[j] = r < mrows && e >= 0 ? m0 + r : -1;
+      if (OP == kLinear && a.rows && arow[j] >= 0) {
+        const int64_t row = a.rows[arow[j]];
+        arow[j] = row < a.T ? row : -1;
+      }
+    }
+  }
+  auto load = [&](int t, gg_u4 (&va)[4], gg_u4 (&vb)[4]) {
+    const int k0 = 64 * t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      va[j] = vb[j] = gg_u4{0u, 0u, 0u, 0u};
+      if constexpr (!TA) {
+        if (arow[j] >= 0) va[j] = gg_load8(A + arow[j] * a.lda, k0 + 8 * (tid & 7), red);
+      } else {
+        const int k = k0 + (tid >> 4) + 16 * j;
+        if (k < red) va[j] = gg_load8(A + (red0 + k) * a.lda + m0, 8 * (tid & 15), mrows);
+      }
+      if constexpr (!TB) {
+        const int r = (tid >> 3) + 32 * j;
+        if (r < ncols) vb[j] = gg_load8(B + (int64_t)e * a.strb + (int64_t)(n0 + r) * a.ldb, k0 + 8 * (tid & 7), red);
+      } else {
+        const int k = k0 + (tid >> 4) + 16 * j;
+        if (k < red) {
+          if constexpr (OP == kDgrad) {
+            vb[j] = gg_load8(B + (int64_t)e * a.strb + (int64_t)k * a.ldb + n0, 8 * (tid & 15), ncols);
+          } else {
+            const int64_t row = a.rows ? a.rows[red0 + k] : red0 + k;
+            if (row >= 0 && row < a.T) vb[j] = gg_load8(B + row * a.ldb + n0, 8 * (tid & 15), ncols);
+          }
+        }
+      }
+    }
+  };
+  auto put = [&](char* img, bool tr, const gg_u4 (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (!tr) {
+        const int r = (tid >> 3) + 32 * j, pos = 64 * (r >> 6) + 8 * (r & 7) + ((r >> 3) & 7);
+        *reinterpret_cast<gg_u4*>(img + pos * 128 + 16 * ((tid & 7) ^ gg_swz(pos))) = v[j];
+      } else {
+        const int k = (tid >> 4) + 16 * j, pos = 8 * (k & 7) + (k >> 3), c = tid & 15;
+        *reinterpret_cast<gg_u4*>(img + (c >> 3) * 8192 + pos * 128 + 16 * ((c & 7) ^ gg_swz_tr(pos))) = v[j];
+      }
+    }
+  };
+  f32x4 acc[XF][YF], accs[2];
+#pragma unroll
+  for (int x = 0; x < XF; ++x)
+#pragma unroll
+    for (int y = 0; y < YF; ++y) acc[x][y] = {0.f, 0.f, 0.f, 0.f};
+  accs[0] = accs[1] = {0.f, 0.f, 0.f, 0.f};
+  const bool sums = OP == kWgrad && a.db && n0 == 0;
+  constexpr uint32_t kOnes = DT == kBF16 ? 0x3f803f80u : 0x3c003c00u;
+  const gg_u4 ones = {kOnes, kOnes, kOnes, kOnes};
+  GgReader<TA, 2> ra;
+  GgReader<TB, 1> rb;
+  ra.init(wr, lane);
+  rb.init(YF * wc, lane);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
+  const int steps = (red + 63) / 64;
+  gg_u4 va[4], vb[4];
+  if (steps > 0) {
+    load(0, va, vb);
+    put(lds, TA, va);
+    put(lds + kImg, TB, vb);
+    if (steps > 1) load(1, va, vb);
+    __syncthreads();
+  }
+  for (int t = 0; t < steps; ++t) {
+    const uint32_t at = lds0 + (t & 1) * 2 * kImg;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      gg_u4 fa[XF], fb[YF];
+#pragma unroll
+      for (int y = 0; y < YF; ++y) fb[y] = gg_frag(rb, at + kImg, h, y);
+#pragma unroll
+      for (int x = 0; x < XF; ++x) fa[x] = gg_frag(ra, at, h, x);
+#pragma unroll
+      for (int x = 0; x < XF; ++x)
+#pragma unroll
+        for (int y = 0; y < YF; ++y) acc[x][y] = gg_mfma<DT>(fb[y], fa[x], acc[x][y]);
+      if (sums) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) accs[u] = gg_mfma<DT>(ones, wc ? fa[2 + u] : fa[u], accs[u]);
+      }
+    }
+    if (t + 1 < steps) {
+      char* to = lds + ((t + 1) & 1) * 2 * kImg;
+      put(to, TA, va);
+      put(to + kImg, TB, vb);
+      if (t + 2 < steps) load(t + 2, va, vb);
+      __syncthreads();
+    }
+  }
+
+  if constexpr (OP == kWgrad) {
+    float* out = static_cast<float*>(a.out) + (int64_t)e * a.stro;
+    if (sums && g == 0) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int m = 16 * (2 * (2 * wc + u) + wr) + i;
+        if (m < mrows) a.db[(int64_t)e * a.N + m0 + m] = accs[u][0];
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      const int m = 16 * (2 * x + wr) + i;
+      if (m >= mrows) continue;
+      float* o = out + (m0 + m) * a.ldo + n0;
+#pragma unroll
+      for (int y = 0; y < YF; ++y) {
+        const int n = wn + 16 * y + 4 * g;
+        if (n + 4 <= ncols) {
+          __builtin_memcpy(o + n, &acc[x][y], 16);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            if (n + q < ncols) o[n + q] = acc[x][y][q];
+        }
+      }
+    }
+  } else {
+    uint16_t* out = static_cast<uint16_t*>(a.out);
+    const uint16_t* mk = OP == kDgrad && e >= 0 ? static_cast<const uint16_t*>(a.mask) : nullptr;
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      const int m = 16 * (2 * x + wr) + i;
+      if (m >= mrows) continue;
+      uint16_t* o = out + (m0 + m) * a.ldo + n0;
+#pragma unroll
+      for (int y = 0; y < YF; ++y) {
+        const int n = wn + 16 * y + 4 * g;
+        f32x4 v = acc[x][y];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (n + q >= ncols) continue;
+          if constexpr (OP == kLinear) {
+            if (e >= 0 && a.bias) v[q] += a.bias[(int64_t)e * a.ldbias + n0 + n + q];
+            if (a.relu) v[q] = v[q] < 0.f ? 0.f : v[q];
+          } else {
+            if (mk && !(gg_f<DT>(mk[(m0 + m) * a.ldmask + n0 + n + q]) > 0.f)) v[q] = 0.f;
+          }
+        }
+        const uint2 u = make_uint2(gg_pack2<DT>(v[0], v[1]), gg_pack2<DT>(v[2], v[3]));
+        if (n + 4 <= ncols) {
+          __builtin_memcpy(o + n, &u, 8);
+        } else {
+          if (n < ncols) o[n] = (uint16_t)u.x;
+          if (n + 1 < ncols) o[n + 1] = (uint16_t)(u.x >> 16);
+          if (n + 2 < ncols) o[n + 2] = (uint16_t)u.y;
+        }
+      }
+    }
+  }
+}
+
+template <int DT>
+hipError_t launch_any(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
+  const int64_t nt = ((op == kLinear ? a.N : a.K) + 127) / 128, some = a.E < a.S ? a.E : a.S;
+  const int64_t mt = op == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
+  const int64_t blocks = (mt * nt + 7) / 8 * 8;
+  if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
+  const dim3 grid((uint32_t)blocks);
+  if (op == kLinear) hipLaunchKernelGGL((grouped_any_k<DT, kLinear>), grid, dim3(256), 0, s, a);
+  else if (op == kDgrad) hipLaunchKernelGGL((grouped_any_k<DT, kDgrad>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((grouped_any_k<DT, kWgrad>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 bool gg_al(const void* p, int64_t ld, int64_t need) {

@@ -33,6 +33,16 @@ SHAPES = [
     ([1030, 520], 512, 768),
 ]
 
+# enough tiles for every kernel: whole rounds of large tiles, their last round
+# and the rows behind them in small ones, more than 64 groups, odd widths
+LARGE = [
+    ([3000, 500, 0, 2600], 1032, 1544),
+    ([97] * 66 + [2500, 0, 1300], 520, 2312),
+    ([1] * 40 + [20000], 264, 520),
+    ([700, 0, 900, 333], 2056, 2056),
+    ([1500, 999], 1037, 1031),
+]
+
 
 def _rand(g, *shape, dt=torch.float32, scale=1.0):
     return (torch.randn(*shape, generator=g, device=DEV) * scale).to(dt)
@@ -47,7 +57,7 @@ def _rows(g, S, T):
 
 
 @pytest.mark.parametrize("dt", [BF, FP])
-@pytest.mark.parametrize("sizes,K,N", SHAPES)
+@pytest.mark.parametrize("sizes,K,N", SHAPES + LARGE)
 @pytest.mark.parametrize("form", ["plain", "bias_relu", "gather"])
 def test_linear(sizes, K, N, dt, form):
     g = _gen(len(sizes) * 1000 + K + N)
@@ -64,7 +74,7 @@ def test_linear(sizes, K, N, dt, form):
 
 
 @pytest.mark.parametrize("dt", [BF, FP])
-@pytest.mark.parametrize("sizes,K,N", SHAPES)
+@pytest.mark.parametrize("sizes,K,N", SHAPES + LARGE)
 @pytest.mark.parametrize("masked", [False, True])
 def test_dgrad(sizes, K, N, dt, masked):
     g = _gen(len(sizes) * 1000 + K + N)
@@ -77,7 +87,7 @@ def test_dgrad(sizes, K, N, dt, masked):
 
 
 @pytest.mark.parametrize("dt", [BF, FP])
-@pytest.mark.parametrize("sizes,K,N", SHAPES)
+@pytest.mark.parametrize("sizes,K,N", SHAPES + LARGE)
 @pytest.mark.parametrize("gather", [False, True])
 def test_wgrad(sizes, K, N, dt, gather):
     g = _gen(len(sizes) * 1000 + K + N)
