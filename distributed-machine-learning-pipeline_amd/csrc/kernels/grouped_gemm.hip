@@ -972,33 +972,41 @@ __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt
 // LDS images; a thread loads 16-B chunks of a step into registers while the
 // step before is multiplied, and stores them into the other buffer after.
 // ---------------------------------------------------------------------------
-// 8 elements from column c of a row that has `limit` of them; 0 behind it.
-__device__ __forceinline__ gg_u4 gg_load8(const uint16_t* row, int c, int limit) {
-  if (c + 8 <= limit) {
-    gg_u4 v;
-    __builtin_memcpy(&v, row + c, 16);
-    return v;
-  }
-  uint64_t lo = 0, hi = 0;
-  if (limit >= 8) {  // the row's last 8, shifted
-    uint64_t v[2];
-    __builtin_memcpy(v, row + (limit - 8), 16);
-    const int sh = c - (limit - 8);
-    if (sh < 4) {
-      lo = (v[0] >> (16 * sh)) | (v[1] << (63 - 16 * sh) << 1);  // sh > 0: the chunk does not fit
-      hi = v[1] >> (16 * sh);
-    } else if (sh < 8) {
-      lo = v[1] >> (16 * (sh - 4));
-    }
-  } else {
+// Loads are never under a condition (the compiler waits for such a load at the
+// end of its branch: 115 us against 58 at 8192 rows, 8 experts of 1003 x 1001):
+// a chunk that does not fit its row is the row's last 8 elements, shifted when
+// it is stored, and one that has no row is some other, zeroed then.
+struct GgChunk {
+  gg_u4 v;
+  int shift;  // elements to drop at the front; 8 or more: all of them
+};
+template <bool NARROW>
+__device__ __forceinline__ void gg_load8(GgChunk& u, const uint16_t* row, int c, int width, bool ok) {
+  if constexpr (!NARROW) {
+    const int at = c < width - 8 ? c : width - 8;
+    __builtin_memcpy(&u.v, row + at, 16);
+    u.shift = ok ? c - at : 8;
+  } else {  // rows that may have fewer than 8
+    uint64_t lo = 0, hi = 0;
 #pragma unroll
-    for (int i = 0; i < 7; ++i)
-      if (c + i < limit) (i < 4 ? lo : hi) |= (uint64_t)row[c + i] << (16 * (i & 3));
+    for (int i = 0; i < 8; ++i)
+      if (c + i < width) (i < 4 ? lo : hi) |= (uint64_t)row[c + i] << (16 * (i & 3));
+    u.v = gg_u4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    u.shift = ok ? 0 : 8;
   }
+}
+__device__ __forceinline__ gg_u4 gg_settle(const GgChunk& u) {
+  uint64_t lo = ((uint64_t)u.v[1] << 32) | u.v[0], hi = ((uint64_t)u.v[3] << 32) | u.v[2];
+  const int s = u.shift & 3;
+  lo = u.shift & 4 ? hi : lo;
+  hi = u.shift & 4 ? 0 : hi;
+  lo = s ? (lo >> (16 * s)) | (hi << (64 - 16 * s)) : lo;
+  hi >>= 16 * s;
+  if (u.shift >= 8) lo = hi = 0;
   return gg_u4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
 }
 
-template <int DT, int OP>
+template <int DT, int OP, bool NARROW>
 __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   constexpr int BM = 128, BN = 128, XF = 4, YF = 4;
   constexpr bool TA = OP == kWgrad, TB = OP != kLinear;
@@ -1019,8 +1027,8 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
     gg_order(pos - e * per, mtb, nt, mi, ni);
     m0 = (int64_t)mi * BM;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
-    red0 = gg_clamp(a.offsets[e], 0, a.S);
-    red = (int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0);
+    red0 = __builtin_amdgcn_readfirstlane((int)gg_clamp(a.offsets[e], 0, a.S));
+    red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
   } else {
     const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
       const int pos = gg_pos(blockIdx.x, mts * nt);
@@ -1030,63 +1038,72 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
       return mi;
     });
     if (t.e == -2) return;
-    e = t.e;
-    m0 = t.s0;
-    mrows = (int)(t.s1 - t.s0);
+    e = __builtin_amdgcn_readfirstlane(t.e);
+    m0 = __builtin_amdgcn_readfirstlane((int)t.s0);
+    mrows = __builtin_amdgcn_readfirstlane((int)(t.s1 - t.s0));
     red = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
   }
-  const int n0 = ni * BN, ncols = cols - n0 < BN ? cols - n0 : BN;
+  const int n0 = __builtin_amdgcn_readfirstlane(ni * BN), ncols = cols - n0 < BN ? cols - n0 : BN;
 
   // chunk q = tid + 256 j of a step: row-major operands row q / 8, chunk q % 8;
   // transposed ones reduction row q / 16, column chunk q % 16
-  int64_t arow[4];  // this thread's rows of a row-major A, -1: none
-  if constexpr (!TA) {
+  struct Set {
+    GgChunk a[4], b[4];
+  };
+  const uint16_t *ap[4], *bp[4];  // row-major: this thread's rows
+  bool ao[4], bo[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = (tid >> 3) + 32 * j;
-      arow[j] = r < mrows && e >= 0 ? m0 + r : -1;
-      if (OP == kLinear && a.rows && arow[j] >= 0) {
-        const int64_t row = a.rows[arow[j]];
-        arow[j] = row < a.T ? row : -1;
+  for (int j = 0; j < 4; ++j) {
+    const int r = (tid >> 3) + 32 * j;
+    if constexpr (!TA) {
+      ao[j] = r < mrows;
+      int64_t row = m0 + (ao[j] ? r : 0);
+      if (OP == kLinear && a.rows && e >= 0) {
+        row = a.rows[row];
+        ao[j] = ao[j] && row >= 0 && row < a.T;
+        row = ao[j] ? row : 0;
       }
+      ap[j] = A + row * a.lda;
+    }
+    if constexpr (!TB) {
+      bo[j] = r < ncols;
+      bp[j] = B + (int64_t)(e < 0 ? 0 : e) * a.strb + (int64_t)(n0 + (bo[j] ? r : 0)) * a.ldb;
     }
   }
-  auto load = [&](int t, gg_u4 (&va)[4], gg_u4 (&vb)[4]) {
+  const bool empty = OP != kDgrad && a.rows && a.T == 0;  // a gather from nothing
+  auto load = [&](int t, Set& u) {
     const int k0 = 64 * t;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      va[j] = vb[j] = gg_u4{0u, 0u, 0u, 0u};
-      if constexpr (!TA) {
-        if (arow[j] >= 0) va[j] = gg_load8(A + arow[j] * a.lda, k0 + 8 * (tid & 7), red);
-      } else {
-        const int k = k0 + (tid >> 4) + 16 * j;
-        if (k < red) va[j] = gg_load8(A + (red0 + k) * a.lda + m0, 8 * (tid & 15), mrows);
-      }
+      const int c = 8 * (tid & 7), k = k0 + (tid >> 4) + 16 * j, kk = k < red ? k : red - 1, m = 8 * (tid & 15);
+      if constexpr (!TA) gg_load8<NARROW>(u.a[j], empty ? B : ap[j], k0 + c, red, ao[j] && !empty);
+      else gg_load8<NARROW>(u.a[j], A + (red0 + kk) * a.lda, (int)m0 + m, a.N, k < red && m < mrows);
       if constexpr (!TB) {
-        const int r = (tid >> 3) + 32 * j;
-        if (r < ncols) vb[j] = gg_load8(B + (int64_t)e * a.strb + (int64_t)(n0 + r) * a.ldb, k0 + 8 * (tid & 7), red);
+        gg_load8<NARROW>(u.b[j], bp[j], k0 + c, red, bo[j]);
+      } else if constexpr (OP == kDgrad) {
+        gg_load8<NARROW>(u.b[j], B + (int64_t)e * a.strb + (int64_t)kk * a.ldb, n0 + m, cols, k < red && m < ncols);
       } else {
-        const int k = k0 + (tid >> 4) + 16 * j;
-        if (k < red) {
-          if constexpr (OP == kDgrad) {
-            vb[j] = gg_load8(B + (int64_t)e * a.strb + (int64_t)k * a.ldb + n0, 8 * (tid & 15), ncols);
-          } else {
-            const int64_t row = a.rows ? a.rows[red0 + k] : red0 + k;
-            if (row >= 0 && row < a.T) vb[j] = gg_load8(B + row * a.ldb + n0, 8 * (tid & 15), ncols);
-          }
+        int64_t row = red0 + kk;
+        bool ok = k < red && m < ncols && !empty;
+        if (a.rows) {
+          row = a.rows[row];
+          ok = ok && row >= 0 && row < a.T;
+          row = ok ? row : 0;
         }
+        gg_load8<NARROW>(u.b[j], empty ? A : B + row * a.ldb, empty ? 0 : n0 + m, empty ? a.N : cols, ok);
       }
     }
   };
-  auto put = [&](char* img, bool tr, const gg_u4 (&v)[4]) {
+  auto put = [&](char* img, bool tr, bool settle, const GgChunk (&u)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      const gg_u4 v = settle ? gg_settle(u[j]) : u[j].v;
       if (!tr) {
         const int r = (tid >> 3) + 32 * j, pos = 64 * (r >> 6) + 8 * (r & 7) + ((r >> 3) & 7);
-        *reinterpret_cast<gg_u4*>(img + pos * 128 + 16 * ((tid & 7) ^ gg_swz(pos))) = v[j];
+        *reinterpret_cast<gg_u4*>(img + pos * 128 + 16 * ((tid & 7) ^ gg_swz(pos))) = v;
       } else {
         const int k = (tid >> 4) + 16 * j, pos = 8 * (k & 7) + (k >> 3), c = tid & 15;
-        *reinterpret_cast<gg_u4*>(img + (c >> 3) * 8192 + pos * 128 + 16 * ((c & 7) ^ gg_swz_tr(pos))) = v[j];
+        *reinterpret_cast<gg_u4*>(img + (c >> 3) * 8192 + pos * 128 + 16 * ((c & 7) ^ gg_swz_tr(pos))) = v;
       }
     }
   };
@@ -1105,15 +1122,19 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   rb.init(YF * wc, lane);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
   const int steps = (red + 63) / 64;
-  gg_u4 va[4], vb[4];
-  if (steps > 0) {
-    load(0, va, vb);
-    put(lds, TA, va);
-    put(lds + kImg, TB, vb);
-    if (steps > 1) load(1, va, vb);
-    __syncthreads();
-  }
-  for (int t = 0; t < steps; ++t) {
+  // whole chunks need no shifting: full tiles of rows that exist, but a last step
+  const bool whole = !NARROW && mrows == BM && ncols == BN && !(OP != kDgrad && a.rows);
+  auto store = [&](int t, const Set& u) {
+    char* to = lds + (t & 1) * 2 * kImg;
+    if (whole && 64 * t + 64 <= red) {
+      put(to, TA, false, u.a);
+      put(to + kImg, TB, false, u.b);
+    } else {
+      put(to, TA, true, u.a);
+      put(to + kImg, TB, true, u.b);
+    }
+  };
+  auto multiply = [&](int t) {
     const uint32_t at = lds0 + (t & 1) * 2 * kImg;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -1131,12 +1152,28 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
         for (int u = 0; u < 2; ++u) accs[u] = gg_mfma<DT>(ones, wc ? fa[2 + u] : fa[u], accs[u]);
       }
     }
-    if (t + 1 < steps) {
-      char* to = lds + ((t + 1) & 1) * 2 * kImg;
-      put(to, TA, va);
-      put(to + kImg, TB, vb);
-      if (t + 2 < steps) load(t + 2, va, vb);
-      __syncthreads();
+  };
+  // step t is multiplied while steps t + 1 (stored after it) and t + 2 are in flight
+  Set u0, u1;
+  if (steps > 0) {
+    load(0, u0);
+    load(steps > 1 ? 1 : 0, u1);
+    store(0, u0);
+    load(steps > 2 ? 2 : 0, u0);
+    __syncthreads();
+    for (int t = 0; t < steps; t += 2) {
+      multiply(t);
+      if (t + 1 < steps) {
+        store(t + 1, u1);
+        if (t + 3 < steps) load(t + 3, u1);
+        __syncthreads();
+        multiply(t + 1);
+        if (t + 2 < steps) {
+          store(t + 2, u0);
+          if (t + 4 < steps) load(t + 4, u0);
+          __syncthreads();
+        }
+      }
     }
   }
 
@@ -1201,16 +1238,15 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   }
 }
 
-template <int DT>
-hipError_t launch_any(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
-  const int64_t nt = ((op == kLinear ? a.N : a.K) + 127) / 128, some = a.E < a.S ? a.E : a.S;
-  const int64_t mt = op == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
+template <int DT, int OP>
+hipError_t launch_any(const GroupedArgs& a, hipStream_t s) {
+  const int64_t nt = ((OP == kLinear ? a.N : a.K) + 127) / 128, some = a.E < a.S ? a.E : a.S;
+  const int64_t mt = OP == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
   const int64_t blocks = (mt * nt + 7) / 8 * 8;
   if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
-  if (op == kLinear) hipLaunchKernelGGL((grouped_any_k<DT, kLinear>), grid, dim3(256), 0, s, a);
-  else if (op == kDgrad) hipLaunchKernelGGL((grouped_any_k<DT, kDgrad>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((grouped_any_k<DT, kWgrad>), grid, dim3(256), 0, s, a);
+  if (a.N < 8 || a.K < 8) hipLaunchKernelGGL((grouped_any_k<DT, OP, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((grouped_any_k<DT, OP, false>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
@@ -1288,6 +1324,11 @@ hipError_t launch_skinny_op(GroupedOp op, const GroupedArgs& a, int mx, hipStrea
 }
 
 template <int DT>
+hipError_t launch_any_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
+  if (op == kLinear) return launch_any<DT, kLinear>(a, s);
+  return op == kDgrad ? launch_any<DT, kDgrad>(a, s) : launch_any<DT, kWgrad>(a, s);
+}
+template <int DT>
 hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
   if (op == kWgrad) return a.rows ? launch_fast<DT, kWgrad, true>(a, s) : launch_fast<DT, kWgrad>(a, s);
   // single tokens: by the mean rows of an expert
@@ -1311,7 +1352,7 @@ hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
     return hipErrorInvalidValue;
   if (op != kWgrad && a.S == 0) return hipSuccess;
   if (fast_ok(op, a)) return a.dtype == kBF16 ? launch_fast_op<kBF16>(op, a, s) : launch_fast_op<kF16>(op, a, s);
-  return a.dtype == kBF16 ? launch_any<kBF16>(op, a, s) : launch_any<kF16>(op, a, s);
+  return a.dtype == kBF16 ? launch_any_op<kBF16>(op, a, s) : launch_any_op<kF16>(op, a, s);
 }
 
 }  // namespace dsml

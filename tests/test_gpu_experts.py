@@ -146,7 +146,7 @@ def test_strided_operands_and_slots_outside_every_group(sizes, K, N, dt):
     assert (buf[:, N] == 7).all() and (buf[:, :, :2] == 7).all() and (buf[:, :, 2 + K:] == 7).all()
 
 
-@pytest.mark.parametrize("K,N", [(24, 40), (264, 520)])
+@pytest.mark.parametrize("K,N", [(24, 40), (264, 520), (25, 39), (5, 130)])
 def test_infinities_and_nan_stay_in_their_rows(K, N):
     """A bad row changes no other row, a bad padding column of a strided operand
     changes nothing, and ReLU keeps a NaN."""
@@ -176,10 +176,11 @@ def test_infinities_and_nan_stay_in_their_rows(K, N):
     assert (X.grouped_dgrad(dz, w, off, m) == 0).all()  # NaN > 0 does not hold
 
 
-def test_plans_out_of_range_stay_in_the_buffers():
+@pytest.mark.parametrize("K,N", [(264, 136), (263, 135), (7, 130), (130, 7)])
+def test_plans_out_of_range_stay_in_the_buffers(K, N):
     """Rows outside x count as zero rows; offsets are clamped to the slots."""
     g = _gen(11)
-    dt, K, N = BF, 264, 136
+    dt = BF
     x, w = _rand(g, 50, K, dt=dt), _rand(g, 2, N, K, dt=dt)
     rows = torch.arange(100, device=DEV, dtype=torch.int32) % 50
     rows[3], rows[60], rows[99] = -1, 50, 2 ** 31 - 1
@@ -197,6 +198,8 @@ def test_plans_out_of_range_stay_in_the_buffers():
     wide = torch.tensor([-5, 40, 10 ** 6], dtype=torch.int32, device=DEV)
     assert torch.equal(X.grouped_linear(x, w, wide, rows=safe), X.grouped_linear(x, w, off, rows=safe))
     assert X.grouped_linear(x[:0], w, off, rows=rows).abs().max() == 0
+    dw, db = X.grouped_wgrad(dz, x[:0], off, rows)
+    assert dw.abs().max() == 0 and torch.equal(db, X.grouped_wgrad(dz, x, off, safe)[1])
 
 
 def test_offsets_past_32_bits():
