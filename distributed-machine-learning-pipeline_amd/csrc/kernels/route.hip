@@ -104,204 +104,206 @@ __device__ __forceinline__ int rt_min(int x) {
   return x;
 }
 
+// Slots of the experts' first choices: exclusive sums of cnt[E] into base[E + 1]
+// (and offsets, by the block that writes them).  One wave.
+__device__ __forceinline__ void rt_offsets(const int* cnt, int* base, int32_t* offsets, int E, bool write) {
+  const int lane = threadIdx.x;
+  int acc = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    const int e = e0 + lane, n = e < E ? cnt[e] : 0;
+    int inc = n;
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x111, 0xf, 0xf, true);  // row_shr 1, 2, 4, 8
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x112, 0xf, 0xf, true);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x114, 0xf, 0xf, true);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x118, 0xf, 0xf, true);
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    inc += __builtin_amdgcn_update_dpp(0, inc, 0x143, 0xc, 0xf, false);
+    if (e < E) {
+      base[e] = acc + inc - n;
+      if (write) offsets[e] = acc + inc - n;
+    }
+    acc += __builtin_amdgcn_readlane(inc, 63);
+  }
+  if (lane == 0) {
+    base[E] = acc;
+    if (write) offsets[E] = acc;
+  }
+}
+
+// Choices of expert e by the tile's tokens before tl (all of them: tl = 256).
+__device__ __forceinline__ int rt_rank(const uint32_t* mask, int e, int tl) {
+  const uint4* m = reinterpret_cast<const uint4*>(mask + 8 * e);
+  const uint4 x = m[0], y = m[1];
+  const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  int r = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int left = tl - 32 * i;
+    r += __popc(left >= 32 ? w[i] : (left > 0 ? w[i] & ((1u << left) - 1u) : 0u));
+  }
+  return r;
+}
+
 // LDS: mask[E][8] words (one bit a token of the tile), run[E] (this block's
-// choices before the tile), base[E] (slot of the block's first choice).
+// choices before the tile), base[E + 1], pick[256 k] (the tile's choices).
 template <int DT, int L>
 __global__ __launch_bounds__(kRtThreads) void route_topk_k(RouteArgs a, int tiles, int vec) {
-  extern __shared__ uint32_t rt_lds[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t rt_lds[];
   uint32_t* mask = rt_lds;
   int* run = reinterpret_cast<int*>(rt_lds + 8 * a.E);
   int* base = run + a.E;
+  int* pick = base + a.E + 1;
   const int tid = threadIdx.x;
-  constexpr int kPer = kRtThreads / L;  // tokens of one pass of the block
+  constexpr int kPer = kRtThreads / L;                                  // tokens of one pass of the block
+  constexpr int kPasses = kRtTile > kPer ? kRtTile / kPer : 1;
+  constexpr int kAhead = kPasses < 4 ? kPasses : 4;                     // rows a lane loads before the first is used
   const int sub = tid % L, c0 = 8 * sub;
   for (int e = tid; e < a.E; e += kRtThreads) run[e] = 0;
   const int64_t t_first = (int64_t)blockIdx.x * tiles * kRtTile;
+  const bool only = gridDim.x == 1;
   for (int tile = 0; tile < tiles; ++tile) {
     const int64_t t0 = t_first + (int64_t)tile * kRtTile;
     if (t0 >= a.T) break;
     const int nt = (int)(a.T - t0 < kRtTile ? a.T - t0 : kRtTile);
-    for (int i = tid; i < 8 * a.E; i += kRtThreads) mask[i] = 0u;
-    __syncthreads();
-    for (int p = 0; p < nt; p += kPer) {
-      const int tl = p + tid / L;
-      if (tl >= nt || tl >= kRtTile) continue;  // whole L-lane groups leave together
-      const int64_t t = t0 + tl;
-      float v[8];
-      rt_row<DT>(a.logits, t * a.ldl, a.E, c0, vec, v);
-      float m = v[0];
+    for (int p0 = 0; p0 < kPasses; p0 += kAhead) {
+      float v[kAhead][8];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
-      m = rt_max<L>(m);
-      const float top = m;
-      float all = 0.f;
-      if (a.all && top > -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) all += expf(v[i] - top);
-        all = rt_sum<L>(all);
+      for (int q = 0; q < kAhead; ++q) {  // a token past the end: the last one's row, not used
+        const int tl = (p0 + q) * kPer + tid / L;
+        rt_row<DT>(a.logits, (t0 + (tl < nt ? tl : nt - 1)) * a.ldl, a.E, c0, vec, v[q]);
       }
-      float den = 0.f;
-      float mine = 0.f;  // lane j of the token keeps choice j's numerator (k > L: in turns)
-      (void)mine;
-      float num[kRouteMaxK];
-      int pick[kRouteMaxK];
+      if (p0 == 0) {
+        for (int i = tid; i < 8 * a.E; i += kRtThreads) mask[i] = 0u;
+        __syncthreads();
+      }
 #pragma unroll
-      for (int j = 0; j < kRouteMaxK; ++j) {
-        if (j >= a.k) break;
-        if (j) {
-          m = v[0];
+      for (int q = 0; q < kAhead; ++q) {
+        const int tl = (p0 + q) * kPer + tid / L;
+        if (tl >= nt) continue;  // whole L-lane groups leave together
+        const int64_t t = t0 + tl;
+        float m = v[q][0];
 #pragma unroll
-          for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
-          m = rt_max<L>(m);
+        for (int i = 1; i < 8; ++i) m = fmaxf(m, v[q][i]);
+        m = rt_max<L>(m);
+        const float top = m;
+        float all = 0.f;
+        if (a.all && top > -INFINITY) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) all += expf(v[q][i] - top);
+          all = rt_sum<L>(all);
         }
-        int at = 0x7fffffff;
+        float den = 0.f;
+        float num[kRouteMaxK];
+        int pk[kRouteMaxK];
 #pragma unroll
-        for (int i = 7; i >= 0; --i) at = v[i] == m ? c0 + i : at;
-        at = rt_min<L>(at);
-        const bool live = m > -INFINITY;
-        pick[j] = live ? at : -1;
-        num[j] = live ? expf(m - top) : 0.f;
-        den += num[j];
+        for (int j = 0; j < kRouteMaxK; ++j) {
+          if (j >= a.k) break;
+          if (j) {
+            m = v[q][0];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c0 + i == at ? -INFINITY : v[i];
-      }
-      const float d = a.all ? all : den;
+            for (int i = 1; i < 8; ++i) m = fmaxf(m, v[q][i]);
+            m = rt_max<L>(m);
+          }
+          int at = 0x7fffffff;
 #pragma unroll
-      for (int j = 0; j < kRouteMaxK; ++j) {
-        if (j >= a.k) break;
-        if (sub == j % L) {
-          a.experts[t * a.k + j] = pick[j];
-          a.gates[t * a.k + j] = pick[j] >= 0 ? num[j] / d : 0.f;
-          if (pick[j] >= 0) atomicOr(&mask[pick[j] * 8 + (tl >> 5)], 1u << (tl & 31));
+          for (int i = 7; i >= 0; --i) at = v[q][i] == m ? c0 + i : at;
+          at = rt_min<L>(at);
+          const bool live = m > -INFINITY;
+          pk[j] = live ? at : -1;
+          num[j] = live ? expf(m - top) : 0.f;
+          den += num[j];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[q][i] = c0 + i == at ? -INFINITY : v[q][i];
+        }
+        const float d = a.all ? all : den;
+#pragma unroll
+        for (int j = 0; j < kRouteMaxK; ++j) {
+          if (j >= a.k) break;
+          if (sub == j % L) {
+            a.experts[t * a.k + j] = pk[j];
+            a.gates[t * a.k + j] = pk[j] >= 0 ? num[j] / d : 0.f;
+            pick[tl * a.k + j] = pk[j];
+            if (pk[j] >= 0) atomicOr(&mask[pk[j] * 8 + (tl >> 5)], 1u << (tl & 31));
+          }
         }
       }
     }
     __syncthreads();
+    if (only) {  // one block, one tile: its counts are the plan
+      for (int e = tid; e < a.E; e += kRtThreads) run[e] = rt_rank(mask, e, kRtTile);
+      __syncthreads();
+      if (tid < 64) rt_offsets(run, base, a.offsets, a.E, true);
+      __syncthreads();
+      const int total = base[a.E];
+      for (int i = tid; i < nt * a.k; i += kRtThreads) {
+        const int e = pick[i], tl = i / a.k;
+        const int s = e >= 0 ? base[e] + rt_rank(mask, e, tl) : -1;
+        a.slots[i] = s;
+        if (s >= 0) a.rows[s] = tl;
+        if (i >= total) a.rows[i] = -1;
+      }
+      return;
+    }
     // rank of every choice in its expert, among this block's choices so far
     for (int i = tid; i < nt * a.k; i += kRtThreads) {
-      const int tl = i / a.k;
-      const int e = a.experts[t0 * a.k + i];
-      int r = -1;
-      if (e >= 0) {
-        r = run[e];
-        const uint32_t* mk = mask + e * 8;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) {
-          const uint32_t bits = w < (tl >> 5) ? mk[w] : (w == (tl >> 5) ? mk[w] & ((1u << (tl & 31)) - 1u) : 0u);
-          r += __popc(bits);
-        }
-      }
-      a.slots[t0 * a.k + i] = r;
+      const int e = pick[i];
+      a.slots[t0 * a.k + i] = e >= 0 ? run[e] + rt_rank(mask, e, i / a.k) : -1;
     }
     __syncthreads();
-    for (int e = tid; e < a.E; e += kRtThreads) {
-      int n = 0;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) n += __popc(mask[e * 8 + w]);
-      run[e] += n;
-    }
+    for (int e = tid; e < a.E; e += kRtThreads) run[e] += rt_rank(mask, e, kRtTile);
     __syncthreads();
   }
-  if (gridDim.x > 1) {
+  if (!only) {
     for (int e = tid; e < a.E; e += kRtThreads) a.counts[(int64_t)blockIdx.x * a.E + e] = run[e];
-    return;
-  }
-  // the only block: offsets, then slots and rows
-  if (tid < 64) {
-    int acc = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 64) {
-      const int e = e0 + tid;
-      const int n = e < a.E ? run[e] : 0;
-      int inc = n;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o);
-        if (tid >= o) inc += u;
-      }
-      if (e < a.E) {
-        base[e] = acc + inc - n;
-        a.offsets[e] = acc + inc - n;
-      }
-      acc += __shfl(inc, 63);
-    }
-    if (tid == 0) {
-      a.offsets[a.E] = acc;
-      base[a.E] = acc;
-    }
-  }
-  __syncthreads();
-  const int total = base[a.E];
-  const int n = (int)(a.T * a.k);
-  for (int i = tid; i < n; i += kRtThreads) {
-    const int e = a.experts[i];
-    if (e >= 0) {
-      const int s = base[e] + a.slots[i];
-      a.slots[i] = s;
-      a.rows[s] = i / a.k;
-    }
-    if (i >= total) a.rows[i] = -1;
+  } else if (a.T == 0) {
+    for (int e = tid; e <= a.E; e += kRtThreads) a.offsets[e] = 0;
   }
 }
 
 // Second launch: block b adds the choices of the blocks before it and of the
-// experts before each, from the whole count table (it is a few KB to 128 KB).
+// experts before each, from the whole count table (it is a few KB to 512 KB).
 __global__ __launch_bounds__(kRtThreads) void route_place_k(RouteArgs a, int tiles, int blocks) {
-  extern __shared__ uint32_t rt_lds[];
+  extern __shared__ __attribute__((aligned(16))) uint32_t rt_lds[];
   int* before = reinterpret_cast<int*>(rt_lds);  // choices of the blocks before, per expert
   int* total = before + a.E;                     // all choices, per expert
   int* base = total + a.E;                       // [E + 1]
   const int tid = threadIdx.x;
-  for (int e = tid; e < a.E; e += kRtThreads) before[e] = total[e] = 0;
-  __syncthreads();
-  // thread = (expert, slice of the blocks): coalesced over experts
-  const int per = kRtThreads / a.E > 0 ? kRtThreads / a.E : 1;
-  for (int i = tid; i < a.E * per; i += kRtThreads) {
-    const int e = i % a.E, q = i / a.E;
-    int sum = 0, bef = 0;
-    for (int b = q; b < blocks; b += per) {
-      const int n = a.counts[(int64_t)b * a.E + e];
-      sum += n;
-      bef += b < (int)blockIdx.x ? n : 0;
-    }
-    atomicAdd(&total[e], sum);  // integers: any order gives the same sum
-    atomicAdd(&before[e], bef);
-  }
-  __syncthreads();
-  if (tid < 64) {
-    int acc = 0;
-    for (int e0 = 0; e0 < a.E; e0 += 64) {
-      const int e = e0 + tid;
-      const int n = e < a.E ? total[e] : 0;
-      int inc = n;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o);
-        if (tid >= o) inc += u;
-      }
-      if (e < a.E) {
-        base[e] = acc + inc - n + before[e];
-        if (blockIdx.x == 0) a.offsets[e] = acc + inc - n;
-      }
-      acc += __shfl(inc, 63);
-    }
-    if (tid == 0) {
-      base[a.E] = acc;
-      if (blockIdx.x == 0) a.offsets[a.E] = acc;
-    }
-  }
-  __syncthreads();
-  const int64_t total_n = base[a.E];
   const int64_t i0 = (int64_t)blockIdx.x * tiles * kRtTile * a.k;
   int64_t i1 = i0 + (int64_t)tiles * kRtTile * a.k;
   if (i1 > a.T * a.k) i1 = a.T * a.k;
+  const int64_t first = i0 + tid < i1 ? i0 + tid : i1 - 1;
+  int e = a.experts[first], r = a.slots[first];  // in flight while the table is summed
+  for (int x = tid; x < a.E; x += kRtThreads) before[x] = total[x] = 0;
+  __syncthreads();
+  // thread = (expert, slice of the blocks): coalesced over experts
+  const int per = kRtThreads / a.E;
+  for (int x = tid; x < a.E * per; x += kRtThreads) {
+    const int ex = x % a.E, q = x / a.E;
+    int sum = 0, bef = 0;
+#pragma unroll 8
+    for (int b = q; b < blocks; b += per) {
+      const int n = a.counts[(int64_t)b * a.E + ex];
+      sum += n;
+      bef += b < (int)blockIdx.x ? n : 0;
+    }
+    atomicAdd(&total[ex], sum);  // integers: any order gives the same sum
+    atomicAdd(&before[ex], bef);
+  }
+  __syncthreads();
+  if (tid < 64) rt_offsets(total, base, a.offsets, a.E, blockIdx.x == 0);
+  __syncthreads();
+  const int64_t all = base[a.E];
   for (int64_t i = i0 + tid; i < i1; i += kRtThreads) {
-    const int e = a.experts[i];
+    if (i != first) {
+      e = a.experts[i];
+      r = a.slots[i];
+    }
     if (e >= 0) {
-      const int s = base[e] + a.slots[i];
+      const int s = base[e] + before[e] + r;
       a.slots[i] = s;
       a.rows[s] = (int32_t)(i / a.k);
     }
-    if (i >= total_n) a.rows[i] = -1;
+    if (i >= all) a.rows[i] = -1;
   }
 }
 
@@ -387,7 +389,7 @@ size_t esize(int dt) { return dt == kF32 ? 4 : 2; }
 
 template <int DT>
 hipError_t launch_topk(const RouteArgs& a, int L, int blocks, int tiles, int vec, hipStream_t s) {
-  const size_t lds = (size_t)(8 * a.E + a.E + a.E + 1) * 4;
+  const size_t lds = (size_t)(8 * a.E + a.E + a.E + 1 + kRtTile * a.k) * 4;
 #define DSML_RT(LL) \
   case LL: hipLaunchKernelGGL((route_topk_k<DT, LL>), dim3(blocks), dim3(kRtThreads), lds, s, a, tiles, vec); break
   switch (L) {
