@@ -57,13 +57,14 @@ __device__ __forceinline__ void cb_unpack(uint4 u, float (&f)[8]) {
   for (int i = 0; i < 8; ++i) f[i] = cb_f<DT>((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
 }
 
-// K: choices held at once (k <= K: one round).  blockIdx.y: column chunk.
+// K: choices held at once (k <= K: one round).  Workgroups next to each other
+// take a row's column chunks in turn: whole rows are read and written together.
 template <int DT, bool VEC, int LPR, int K>
-__global__ __launch_bounds__(kCbThreads) void combine_k(CombineArgs a) {
-  const int sub = threadIdx.x % LPR;
-  const int64_t t = (int64_t)blockIdx.x * (kCbThreads / LPR) + threadIdx.x / LPR;
+__global__ __launch_bounds__(kCbThreads) void combine_k(CombineArgs a, int chunks) {
+  const int sub = threadIdx.x % LPR, chunk = blockIdx.x % chunks;
+  const int64_t t = (int64_t)(blockIdx.x / chunks) * (kCbThreads / LPR) + threadIdx.x / LPR;
   if (t >= a.T) return;
-  const int c = 8 * (blockIdx.y * LPR + sub);
+  const int c = 8 * (chunk * LPR + sub);
   if (c >= a.N) return;
   float acc[8];
 #pragma unroll
@@ -177,11 +178,13 @@ bool al16(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 
 
 template <int DT, bool VEC, int LPR>
 hipError_t launch_combine(const CombineArgs& a, hipStream_t s) {
-  const int per = kCbThreads / LPR;
-  const dim3 grid((uint32_t)((a.T + per - 1) / per), (a.N + 8 * LPR - 1) / (8 * LPR));
-  if (a.k == 1) hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 1>), grid, dim3(kCbThreads), 0, s, a);
-  else if (a.k == 2) hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 2>), grid, dim3(kCbThreads), 0, s, a);
-  else hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 4>), grid, dim3(kCbThreads), 0, s, a);
+  const int per = kCbThreads / LPR, chunks = (a.N + 8 * LPR - 1) / (8 * LPR);
+  const int64_t blocks = (a.T + per - 1) / per * chunks;
+  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  const dim3 grid((uint32_t)blocks);
+  if (a.k == 1) hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 1>), grid, dim3(kCbThreads), 0, s, a, chunks);
+  else if (a.k == 2) hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 2>), grid, dim3(kCbThreads), 0, s, a, chunks);
+  else hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 4>), grid, dim3(kCbThreads), 0, s, a, chunks);
   return hipGetLastError();
 }
 template <int DT, bool VEC, int LPR>

@@ -310,20 +310,33 @@ __global__ __launch_bounds__(kRtThreads) void route_place_k(RouteArgs a, int til
 // dlogits: one token in L lanes, as above.
 //   chosen-normalised: dl_j = g_j (dg_j - sum_i g_i dg_i) at the chosen experts, else 0
 //   row-normalised:    dl_e = [chosen] g_e dg_e - p_e sum_i g_i dg_i,  p = softmax(row)
-template <int DT, int L>
+// K: at least k; every load of the token is requested before the first is used.
+template <int DT, int L, int K>
 __global__ __launch_bounds__(256) void route_bwd_k(RouteBwdArgs a, int vec, int ovec) {
   const int sub = threadIdx.x % L, c0 = 8 * sub;
   const int64_t t = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   if (t >= a.T) return;  // whole L-lane groups leave together
+  int e[K];
+  float g[K], u[K];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    const int64_t at = t * a.k + (j < a.k ? j : 0);
+    e[j] = a.experts[at];
+    g[j] = a.gates[at];
+    u[j] = a.dgates[at];
+  }
+  float v[8];
+  if (a.all) rt_row<DT>(a.logits, t * a.ldl, a.E, c0, vec, v);
   float inner = 0.f;
-  for (int j = 0; j < a.k; ++j)
-    if (a.experts[t * a.k + j] >= 0) inner += a.gates[t * a.k + j] * a.dgates[t * a.k + j];
+#pragma unroll
+  for (int j = 0; j < K; ++j) {
+    if (j >= a.k) e[j] = -1;
+    if (e[j] >= 0) inner += g[j] * u[j];
+  }
   float d[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) d[i] = 0.f;
   if (a.all) {
-    float v[8];
-    rt_row<DT>(a.logits, t * a.ldl, a.E, c0, vec, v);
     float m = v[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
@@ -341,12 +354,11 @@ __global__ __launch_bounds__(256) void route_bwd_k(RouteBwdArgs a, int vec, int 
       for (int i = 0; i < 8; ++i) d[i] = -v[i] * f;
     }
   }
-  for (int j = 0; j < a.k; ++j) {
-    const int e = a.experts[t * a.k + j];
-    const float g = a.gates[t * a.k + j], dg = a.dgates[t * a.k + j];
-    const float u = a.all ? g * dg : g * (dg - inner);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) d[i] += e == c0 + i ? u : 0.f;
+  for (int j = 0; j < K; ++j) {
+    const float w = g[j] * (a.all ? u[j] : u[j] - inner);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] += e[j] == c0 + i ? w : 0.f;
   }
   if (c0 >= a.E) return;
   const int64_t o = t * a.E + c0;
@@ -399,17 +411,24 @@ hipError_t launch_topk(const RouteArgs& a, int L, int blocks, int tiles, int vec
 #undef DSML_RT
   return hipGetLastError();
 }
-template <int DT>
+template <int DT, int K>
 hipError_t launch_bwd(const RouteBwdArgs& a, int L, int vec, int ovec, hipStream_t s) {
   const int64_t per = 256 / L, blocks = (a.T + per - 1) / per;
 #define DSML_RT(LL) \
-  case LL: hipLaunchKernelGGL((route_bwd_k<DT, LL>), dim3((uint32_t)blocks), dim3(256), 0, s, a, vec, ovec); break
+  case LL: hipLaunchKernelGGL((route_bwd_k<DT, LL, K>), dim3((uint32_t)blocks), dim3(256), 0, s, a, vec, ovec); break
   switch (L) {
     DSML_RT(1); DSML_RT(2); DSML_RT(4); DSML_RT(8); DSML_RT(16); DSML_RT(32); DSML_RT(64);
     default: return hipErrorInvalidValue;
   }
 #undef DSML_RT
   return hipGetLastError();
+}
+
+template <int DT>
+hipError_t launch_bwd_k(const RouteBwdArgs& a, int L, int vec, int ovec, hipStream_t s) {
+  if (a.k <= 2) return launch_bwd<DT, 2>(a, L, vec, ovec, s);
+  if (a.k <= 8) return launch_bwd<DT, 8>(a, L, vec, ovec, s);
+  return launch_bwd<DT, kRouteMaxK>(a, L, vec, ovec, s);
 }
 
 bool route_ok(int64_t T, int E, int k) {
@@ -446,9 +465,9 @@ hipError_t route_topk_backward(const RouteBwdArgs& a, hipStream_t s) {
   const int ovec = a.E % 8 == 0 && (reinterpret_cast<uintptr_t>(a.dlogits) & 15) == 0;
   const int L = rt_lanes(a.E);
   switch (a.dtype) {
-    case kF32: return launch_bwd<kF32>(a, L, vec, ovec, s);
-    case kBF16: return launch_bwd<kBF16>(a, L, vec, ovec, s);
-    case kF16: return launch_bwd<kF16>(a, L, vec, ovec, s);
+    case kF32: return launch_bwd_k<kF32>(a, L, vec, ovec, s);
+    case kBF16: return launch_bwd_k<kBF16>(a, L, vec, ovec, s);
+    case kF16: return launch_bwd_k<kF16>(a, L, vec, ovec, s);
     default: return hipErrorInvalidValue;
   }
 }
