@@ -8,9 +8,10 @@
 // waits for bytes, not for arithmetic).  Two passes: the first leaves one fp64
 // partial per workgroup, every workgroup of the second sums all of them in
 // the same order -- no atomics, so the result does not depend on timing -- and
-// scales its share.  Tensors are cut into pieces of 4096 16-B words; a
-// workgroup takes every gridDim-th piece.  The tensor table travels in the
-// kernel arguments, so a call keeps nothing on the device and can be captured.
+// scales its share.  Tensors are cut into pieces of 256 to 4096 16-B words (about
+// 1024 pieces in all, each thread's words of one requested together); a workgroup
+// takes every gridDim-th piece.  The tensor table travels in the kernel
+// arguments, so a call keeps nothing on the device and can be captured.
 #include <algorithm>
 
 #include "common.h"
@@ -22,7 +23,6 @@ namespace {
 
 constexpr int kGnThreads = 256;
 constexpr int kGnMax = 128;            // tensors of one launch (3.6 KB of arguments)
-constexpr int kGnPiece = 4096;         // 16-B words of one piece
 constexpr int kGnBlocks = 1024;        // workgroups over all launches, about
 
 struct GnTable {
@@ -31,6 +31,7 @@ struct GnTable {
   int64_t n[kGnMax];
   uint32_t start[kGnMax + 1];  // first piece of each tensor
   int count;
+  int piece;  // 16-B words
 };
 
 template <int DT>
@@ -70,15 +71,33 @@ __device__ __forceinline__ uint4 gn_pack(const float (&f)[gn_per<DT>()]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Tensor of piece p (uniform over the workgroup).
+// Tensor of piece p.  The lanes look at all the starts at once: the arguments
+// lie in memory, and a search would wait for them once a halving.
 __device__ __forceinline__ int gn_find(const GnTable& t, uint32_t p) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (t.start[mid] <= p) lo = mid;
-    else hi = mid - 1;
+  const int lane = threadIdx.x & 63;
+  const GnTable* k = (const GnTable*)__builtin_amdgcn_kernarg_segment_ptr();  // t is the first argument
+  int at = 0;
+#pragma unroll
+  for (int i = 0; i < kGnMax; i += 64) {
+    const bool before = i + lane < t.count && k->start[i + lane] <= p;
+    at += __popcll(__ballot(before));
   }
-  return lo;
+  return __builtin_amdgcn_readfirstlane(at - 1);
+}
+
+// f(k) for this thread's 16-B words k of a piece, [first, last) in elements of
+// which whole words are [k0, k1); U words in flight.
+template <int U, class Load, class Use>
+__device__ __forceinline__ void gn_words(int64_t k0, int64_t k1, Load load, Use use) {
+  int64_t k = k0 + threadIdx.x;
+  for (; k + (U - 1) * kGnThreads < k1; k += U * kGnThreads) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = load(k + u * kGnThreads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) use(k + u * kGnThreads, v[u]);
+  }
+  for (; k < k1; k += kGnThreads) use(k, load(k));
 }
 
 __device__ __forceinline__ double gn_block_sum(double v, double* lds) {
@@ -103,17 +122,17 @@ __global__ __launch_bounds__(kGnThreads) void grad_sq_k(GnTable t, double* part)
   for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
     const int i = gn_find(t, p);
     const void* g = t.g[i];
-    const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * kGnPiece * P;
-    const int64_t last = first + (int64_t)kGnPiece * P < n ? first + (int64_t)kGnPiece * P : n;
+    const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * t.piece * P;
+    const int64_t last = first + (int64_t)t.piece * P < n ? first + (int64_t)t.piece * P : n;
     if ((reinterpret_cast<uintptr_t>(g) & 15) == 0) {
       const uint4* v = reinterpret_cast<const uint4*>(g);
       const int64_t v1 = last / P;
-      for (int64_t k = first / P + threadIdx.x; k < v1; k += kGnThreads) {
+      gn_words<8>(first / P, v1, [&](int64_t k) { return v[k]; }, [&](int64_t, uint4 u) {
         float f[P];
-        gn_unpack<DT>(v[k], f);
+        gn_unpack<DT>(u, f);
 #pragma unroll
         for (int j = 0; j < P; ++j) acc = fma((double)f[j], (double)f[j], acc);
-      }
+      });
       for (int64_t k = v1 * P + threadIdx.x; k < last; k += kGnThreads) {
         const double x = gn_ld<DT>(g, k);
         acc = fma(x, x, acc);
@@ -158,19 +177,19 @@ __global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const doub
     const void* g = t.g[i];
     void* o = t.out[i];
     if (c == 1.f && o == g) continue;  // nothing changes
-    const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * kGnPiece * P;
-    const int64_t last = first + (int64_t)kGnPiece * P < n ? first + (int64_t)kGnPiece * P : n;
+    const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * t.piece * P;
+    const int64_t last = first + (int64_t)t.piece * P < n ? first + (int64_t)t.piece * P : n;
     if (((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
       const uint4* v = reinterpret_cast<const uint4*>(g);
       uint4* w = reinterpret_cast<uint4*>(o);
       const int64_t v1 = last / P;
-      for (int64_t k = first / P + threadIdx.x; k < v1; k += kGnThreads) {
+      gn_words<8>(first / P, v1, [&](int64_t k) { return v[k]; }, [&](int64_t k, uint4 u) {
         float f[P];
-        gn_unpack<DT>(v[k], f);
+        gn_unpack<DT>(u, f);
 #pragma unroll
         for (int j = 0; j < P; ++j) f[j] *= c;
         w[k] = gn_pack<DT>(f);
-      }
+      });
       for (int64_t k = v1 * P + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, gn_ld<DT>(g, k) * c);
     } else {
       for (int64_t k = first + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, gn_ld<DT>(g, k) * c);
@@ -178,9 +197,14 @@ __global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const doub
   }
 }
 
-int64_t gn_pieces(int64_t n, int P) {
-  const int64_t per = (int64_t)kGnPiece * P;
+int64_t gn_pieces(int64_t n, int P, int piece) {
+  const int64_t per = (int64_t)piece * P;
   return (n + per - 1) / per;
+}
+// 16-B words of a piece: about 1024 pieces, whole rounds of the threads.
+int gn_piece(int64_t words) {
+  const int64_t w = (words / kGnBlocks + kGnThreads - 1) / kGnThreads * kGnThreads;
+  return (int)std::min<int64_t>(4096, std::max<int64_t>(kGnThreads, w));
 }
 // Workgroups of one launch: its share of the pieces of the whole call.
 int gn_grid(int64_t pieces, int64_t all) {
@@ -201,23 +225,26 @@ template <int DT>
 static hipError_t run_norm(const ClipTensor* t, int count, double* ws, float* norm, bool clip, double max_norm,
                            double eps, hipStream_t s) {
   constexpr int P = gn_per<DT>();
-  int64_t all = 0;
+  int64_t all = 0, words = 0;
+  for (int i = 0; i < count; ++i) words += t[i].n / P;
+  const int piece = gn_piece(words);
   for (int i = 0; i < count; ++i) {
-    if (t[i].n < 0 || gn_pieces(t[i].n, P) > 0x3fffffffLL) return hipErrorInvalidValue;
-    all += gn_pieces(t[i].n, P);
+    if (t[i].n < 0 || gn_pieces(t[i].n, P, piece) > 0x3fffffffLL) return hipErrorInvalidValue;
+    all += gn_pieces(t[i].n, P, piece);
   }
   int parts = 0;
   for (int pass = 0; pass < (clip ? 2 : 1); ++pass) {
     for (int i0 = 0; i0 < count; i0 += kGnMax) {
       GnTable tb;
       tb.count = std::min(kGnMax, count - i0);
+      tb.piece = piece;
       int64_t pieces = 0;
       for (int i = 0; i < tb.count; ++i) {
         tb.g[i] = t[i0 + i].g;
         tb.out[i] = t[i0 + i].out;
         tb.n[i] = t[i0 + i].n;
         tb.start[i] = (uint32_t)pieces;
-        pieces += gn_pieces(t[i0 + i].n, P);
+        pieces += gn_pieces(t[i0 + i].n, P, piece);
         if (pieces > 0x7fffffffLL) return hipErrorInvalidValue;
       }
       tb.start[tb.count] = (uint32_t)pieces;
