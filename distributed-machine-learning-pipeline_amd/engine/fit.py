@@ -70,7 +70,7 @@ def build_trainer(cfg: TrainConfig, spec: MlpSpec, data: Dataset, ctx: DistConte
                               # kernels; the wide engine syncs by RCCL
                               sync="rccl" if cfg.sync in ("auto", "xact", "xgmi", "pk", "pk2", "pkg", "pkg2",
                                                           "pkx") else cfg.sync,
-                              graph=cfg.graph_steps != 0), engine
+                              graph=cfg.graph_steps != 0, clip_norm=cfg.clip_norm), engine
     from .trainer import MlpTrainer
 
     # graphs replay the fused-exchange steps too; a step with an RCCL collective
@@ -79,7 +79,7 @@ def build_trainer(cfg: TrainConfig, spec: MlpSpec, data: Dataset, ctx: DistConte
     return MlpTrainer(spec, data, batch=cfg.batch, lr=cfg.lr, ctx=ctx, seed=cfg.seed,
                       init="reference" if cfg.init == "auto" else cfg.init, momentum=cfg.momentum,
                       weight_decay=cfg.weight_decay, sync=cfg.sync,
-                      ring_chunk_bytes=cfg.ring_chunk_bytes, graph_steps=gs), engine
+                      ring_chunk_bytes=cfg.ring_chunk_bytes, graph_steps=gs, clip_norm=cfg.clip_norm), engine
 
 
 def _fault_hook(ctx: DistContext, step: int) -> None:

@@ -85,6 +85,8 @@ def _pad_cols(X: torch.Tensor, mult: int = 4) -> torch.Tensor:
 
 
 class MlpTrainer:
+    clip_norm: float = 0.0
+
     def __init__(self, spec: MlpSpec, data: Dataset, batch: int = 64, lr: float = 0.01, *,
                  ctx: Optional[DistContext] = None, seed: int = 0, init: str = "reference",
                  momentum: float = 0.0, weight_decay: float = 0.0, sync: str = "rccl",
@@ -95,7 +97,7 @@ class MlpTrainer:
                  stream: Optional["torch.cuda.Stream"] = None, persist: Optional[bool] = None,
                  grad_allreduce=None, node_local: Optional[bool] = None,
                  persist_place_trials: Optional[int] = None,
-                 init_phases: Optional[InitPhases] = None):
+                 init_phases: Optional[InitPhases] = None, clip_norm: float = 0.0):
         if sync not in SYNC_MODES:
             raise ValueError(f"sync must be one of {SYNC_MODES}")
         self.ctx = ctx or DistContext()
@@ -108,6 +110,14 @@ class MlpTrainer:
         self.lr = float(lr)
         self.momentum = float(momentum)
         self.weight_decay = float(weight_decay)
+        # > 0: the averaged gradient's global norm is clipped to this before the
+        # update, which then cannot be fused into the weight-gradient kernels
+        if not clip_norm >= 0:
+            raise ValueError(f"clip_norm must not be negative, got {clip_norm}")
+        self.clip_norm = float(clip_norm)
+        if self.clip_norm and sync in EXCHANGE_MODES:
+            raise ValueError(f"sync='{sync}' applies the update inside the exchange; use rccl, ring or "
+                             "torch with clip_norm")
         self.sync = sync
         self.graph_steps = int(graph_steps)
         if len(data) < self.batch:
@@ -219,7 +229,7 @@ class MlpTrainer:
         # send/recv pairs of the in-house ring -- tracked per mode
         self._warm_modes: set = set()
         if not self.ctx.is_distributed:
-            plain = not (self.momentum or self.weight_decay)
+            plain = not (self.momentum or self.weight_decay or self.clip_norm)
             if self._want_persist and plain and C.mlp_persist_supported(self.layout.desc_list()):
                 self.pk_buf = torch.zeros(C.mlp_persist_xbuf_granules(), dtype=torch.int64, device=d)
                 self.pk_err = torch.zeros(1, dtype=torch.int32, device=d)
@@ -280,7 +290,7 @@ class MlpTrainer:
         an eligible group, see _xgmi_eligible)."""
         if self.sync in EXCHANGE_MODES:
             return [self.sync]
-        plain = not (self.momentum or self.weight_decay)
+        plain = not (self.momentum or self.weight_decay or self.clip_norm)
         if not (self.sync == "auto" and plain and _xgmi_eligible(self.ctx, self._node_local)):
             return []
         # pk2 pays one more flag round trip per slot for fewer bytes: a
@@ -573,6 +583,36 @@ class MlpTrainer:
                 dist.all_reduce(self.G)
             self.runner.update()
 
+    def _clip(self, g: torch.Tensor) -> None:
+        """Clip the replicas' summed gradient so that their mean's global norm is
+        at most clip_norm."""
+        from ..ops.functional import clip_grad_norm_
+
+        world = self.ctx.world_size
+        clip_grad_norm_([g], self.clip_norm * world, eps=1e-6 * world)
+
+    def _hip_step_clipped(self, n: int) -> None:
+        """Gradient, all-reduce, clipping and update as separate launches on the
+        runner's stream."""
+        import torch.distributed as dist
+
+        if self.runner.follows_torch:
+            stream = torch.cuda.current_stream(self.device)
+        else:
+            stream = torch.cuda.ExternalStream(self.runner.stream_handle(), device=self.device)
+        for _ in range(n):
+            self.runner.fwd_bwd()
+            with torch.cuda.stream(stream):
+                if self.ctx.is_distributed:
+                    if self.sync_active == "ring":
+                        self.comm.ring_allreduce_(self.G, 0, self._ring_chunk)
+                    elif self.sync_active == "rccl":
+                        self.comm.allreduce_(self.G, 0)
+                    else:
+                        dist.all_reduce(self.G)
+                self._clip(self.G)
+            self.runner.update()
+
     # -------------------------------------------------------------- public --
     @property
     def persistent(self) -> bool:
@@ -651,7 +691,7 @@ class MlpTrainer:
 
     def _graphs_on(self) -> bool:
         """Whether train_steps replays hipGraphs for the active sync mode."""
-        if self.graph_steps <= 0 or self.runner is None or self.persistent:
+        if self.graph_steps <= 0 or self.runner is None or self.persistent or self.clip_norm:
             return False
         if not self.ctx.is_distributed:
             return True
@@ -690,7 +730,9 @@ class MlpTrainer:
                 self._torch_step()
                 self.steps_done += 1
             return
-        if self.ctx.is_distributed and self.sync_active == "torch":
+        if self.clip_norm:
+            self._hip_step_clipped(n)
+        elif self.ctx.is_distributed and self.sync_active == "torch":
             self._hip_step_torch_sync(n)
         elif self._graphs_on():
             self.steps_done += n
@@ -858,6 +900,8 @@ class MlpTrainer:
 
             with self.ctx.guard("gradient all_reduce"):
                 dist.all_reduce(g)
+        if self.clip_norm:
+            self._clip(g)
         if self.momentum or self.weight_decay:
             gg = g / world + self.weight_decay * self.P
             self.V.mul_(self.momentum).add_(gg)

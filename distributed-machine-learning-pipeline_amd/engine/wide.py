@@ -60,10 +60,13 @@ def _rup(x: int, m: int) -> int:
 
 
 class WideMlpTrainer:
+    clip_norm: float = 0.0
+
     def __init__(self, spec: MlpSpec, data: Dataset, batch: int = 64, lr: float = 0.01, *,
                  ctx: Optional[DistContext] = None, seed: int = 0, init: str = "kaiming",
                  sync: str = "rccl", target_wgs: int = 256, graph: bool = True,
-                 gemm: str = "skinny", serial_sync: bool = False, xblk: Optional[bool] = None):
+                 gemm: str = "skinny", serial_sync: bool = False, xblk: Optional[bool] = None,
+                 clip_norm: float = 0.0):
         from ..ops.native import require_native
 
         self.C = require_native()
@@ -79,6 +82,13 @@ class WideMlpTrainer:
         if sync not in ("rccl", "ring", "torch", "xact"):
             raise ValueError("sync must be 'rccl', 'ring', 'torch' (gradient all-reduce) or 'xact' "
                              "(activation all-gather)")
+        if not clip_norm >= 0:
+            raise ValueError(f"clip_norm must not be negative, got {clip_norm}")
+        if clip_norm and sync == "xact":
+            raise ValueError("sync='xact' forms no gradient to clip; use rccl, ring or torch with clip_norm")
+        # > 0: the averaged gradient's global norm is clipped to this; the step
+        # then writes every gradient before any update (no fused SGD)
+        self.clip_norm = float(clip_norm)
         if gemm not in ("skinny", "rows64"):
             raise ValueError("gemm must be 'skinny' (split-K 64x64 tiles) or 'rows64' (full-K "
                              "64x16 tiles) for the forward products")
@@ -196,7 +206,7 @@ class WideMlpTrainer:
         # update of W_1 while the next one is written); _carry is the step whose
         # H_1 is already in its buffer (None: run the forward first).
         self.fused_input = (os.environ.get("HIPDSML_WIDE_FUSED_INPUT", "1") == "1" and not self.ctx.is_distributed
-                            and L >= 3 and batch == 64 and d[0] % 16 == 0 and d[0] <= 1024 and d[1] % 64 == 0
+                            and not self.clip_norm and L >= 3 and batch == 64 and d[0] % 16 == 0 and d[0] <= 1024 and d[1] % 64 == 0
                             and self.head_slabs and self.plans["b1"][4] <= 8 and self.pd[0] == d[0])
         self._carry: Optional[int] = None
         self._input_beside = os.environ.get("HIPDSML_WIDE_INPUT_BESIDE", "1") == "1"
@@ -386,7 +396,7 @@ class WideMlpTrainer:
             C.softmax_xent(self.logits, self.y[r0:r0 + Bt], Bt, d[L], 1.0 / Bt, self.dZ[L],
                            None, self.stats)
         world = self.ctx.world_size
-        fused_sgd = world == 1
+        fused_sgd = world == 1 and not self.clip_norm
         scale = self.lr / world
         main = torch.cuda.current_stream(self.device)
         if self.xact:
@@ -467,8 +477,24 @@ class WideMlpTrainer:
             self._sync_layer(l, scale, cur[l], nxt[l])
         # join: the next step's forward reads every updated layer (and overwrites
         # the activations the comm-stream updates read)
-        main.wait_stream(self._cs)
+        if self._cs is not None:
+            main.wait_stream(self._cs)
+        if self.clip_norm:
+            # every layer's gradient is in G (its padding is zero) and nothing has
+            # been updated yet: clip, then step
+            from ..ops.functional import clip_grad_norm_
+
+            clip_grad_norm_([self.G], self.clip_norm * world, eps=1e-6 * world)
+            for l in range(L):
+                self._update_layer(l, scale, cur[l], nxt[l])
         self.steps_done += 1
+
+    def _update_layer(self, l: int, scale: float, wb_cur: torch.Tensor, wb_next: torch.Tensor) -> None:
+        """W_l and b_l -= scale * G, the refreshed bf16 copy into `wb_next`."""
+        _, b = self.views[l]
+        gW, gb = self.gviews[l]
+        self.C.hilo_sgd(wb_cur, self.Wlo[l], gW, scale, wb_next)
+        self.C.sgd_update_(b, gb, scale)
 
     def _sync_layer(self, l: int, scale: float, wb_cur: torch.Tensor, wb_next: torch.Tensor) -> None:
         """Per-layer gradient bucket: as soon as layer l's weight gradient is
@@ -476,13 +502,13 @@ class WideMlpTrainer:
         while the backward of layers < l continues on the compute stream (none of
         them reads W_l or the bf16 copy being written).  Buckets are whole
         layers, issued in the same order on every rank.  The refreshed bf16
-        copy goes to the parity buffer the NEXT step reads."""
-        C, d = self.C, self.spec.dims
+        copy goes to the parity buffer the NEXT step reads.  With clip_norm only the
+        all-reduce happens here: no layer may step before all are reduced."""
+        if not self.ctx.is_distributed:
+            return  # clipping alone: nothing to reduce, the update follows the clip
         main = torch.cuda.current_stream(self.device)
         cs = main if self.serial_sync else self._cs
         cs.wait_stream(main)
-        W, b = self.views[l]
-        gW, gb = self.gviews[l]
         lo, hi = self._gspan[l]
         with torch.cuda.stream(cs):
             if self._comm_delay_cycles:
@@ -495,8 +521,8 @@ class WideMlpTrainer:
                 import torch.distributed as dist
 
                 dist.all_reduce(g)
-            C.hilo_sgd(wb_cur, self.Wlo[l], gW, scale, wb_next)
-            C.sgd_update_(b, gb, scale)
+            if not self.clip_norm:
+                self._update_layer(l, scale, wb_cur, wb_next)
 
     def _warm_comm(self) -> None:
         """Every bucket's collective once, eagerly, before any capture: RCCL

@@ -35,6 +35,7 @@ class TrainConfig:
     lr: float = 0.01                      # client.go:27
     momentum: float = 0.0
     weight_decay: float = 0.0
+    clip_norm: float = 0.0                # > 0: clip the gradient's global norm to this before the update
     epochs: int = 10                      # client.go:28
     steps: int = 0                        # >0: stop after this many steps (overrides epochs)
     init: str = "auto"                    # reference: U(-0.05, 0.05) (client.go:44-51) | kaiming;
