@@ -57,8 +57,7 @@ struct GroupedArgs {
   int64_t ldmask;
   void* out;  // linear: [S][ldo] (N columns); dgrad: [S][ldo] (K columns); wgrad: fp32 [E][N][K]
   int64_t ldo, stro;
-  float* db;    // wgrad: fp32 [E][N], or null
-  float* ws;    // split workspace (grouped_ws_floats)
+  float* db;  // wgrad: fp32 [E][N], or null
   int64_t S, T;  // slots, rows of x
   int E, N, K;
   int dtype;  // kBF16 or kF16
@@ -66,7 +65,6 @@ struct GroupedArgs {
   int zero_rest;  // rows of out in no group are zeroed (else left as they were)
 };
 enum GroupedOp : int { kLinear = 0, kDgrad = 1, kWgrad = 2 };
-int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a);
 hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s);
 
 // ---- gated sum of a token's expert rows -------------------------------------

@@ -44,11 +44,6 @@ __device__ __forceinline__ float gg_f(uint16_t h) {
   if constexpr (DT == kBF16) return bf16_to_f32(h);
   else return __half2float(__ushort_as_half(h));
 }
-template <int DT>
-__device__ __forceinline__ uint16_t gg_h(float v) {
-  if constexpr (DT == kBF16) return f32_to_bf16(v);
-  else return __half_as_ushort(__float2half(v));
-}
 
 struct GgTile {
   int e;          // expert, -1: rows to zero, -2: nothing
@@ -67,6 +62,8 @@ __device__ __forceinline__ int gg_scan64(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31 into rows 2 and 3
   return v;
 }
+
+constexpr int kGgZero = 128;  // workgroups that clear rows of no group
 
 // The groups, cut into tiles on the GPU: count(rows) is what a group of that
 // many rows holds of some kind of tile.  One wave scan per 64 experts, done by
@@ -138,6 +135,17 @@ struct GgGroups {
     hi = t < hn ? h : S;
     hi = lo + BM < hi ? lo + BM : hi;
     return lo < hi;
+  }
+  // All of them at once, by kGgZero workgroups of 256 (whole 16-B words): a row
+  // tile each would be S / 128 column strips of workgroups that mostly end at
+  // once (27 us at 32768 rows of 4096 columns).
+  __device__ __forceinline__ void zero_rest(const GroupedArgs& a, int cols, int part) const {
+    const int64_t h = gg_clamp(off[0], 0, S), n = h + S - gg_clamp(off[E], h, S);
+    const int words = cols / 8, step = kGgZero * 256 / 64, lane = threadIdx.x & 63;
+    for (int64_t r = part * 4 + (threadIdx.x >> 6); r < n; r += step) {
+      uint16_t* o = static_cast<uint16_t*>(a.out) + (r < h ? r : S - n + r) * a.ldo;
+      for (int c = lane; c < words; c += 64) reinterpret_cast<uint4*>(o)[c] = make_uint4(0, 0, 0, 0);
+    }
   }
 };
 
@@ -443,7 +451,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
   const int cols = OP == kLinear ? a.N : a.K;
 
   // ---- which tile ----
-  int e, mrows;           // expert (-1: rows to zero), rows of this tile
+  int e, mrows;           // expert, rows of this tile
   int64_t m0, red0 = 0;   // first output row; first reduction row (wgrad)
   int red;                // reduction length
   int n0;
@@ -476,6 +484,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
     red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
   } else {
     const GgGroups gr(a.offsets, a.E, a.S);
+    if (kSmall && a.zero_rest && blockIdx.x >= gridDim.x - kGgZero) {
+      gr.zero_rest(a, cols, blockIdx.x - (gridDim.x - kGgZero));
+      return;
+    }
     const int nts = (cols + 127) / 128;
     const GgPlan pl = gg_plan(gr, ntb, nts, ((OP == kLinear ? a.K : a.N) + 63) / 64, big < 0);
     int mi, ni;
@@ -486,9 +498,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
       if (!gg_rows(gr, pl, mi, e, m0, mrows)) return;
       n0 = ni * 256;
     } else {
-      int head = 0, tail = 0;
-      if (a.zero_rest) gr.rest(head, tail, 128);
-      const int quarters = 4 * (pl.mt * ntb - pl.big), mts = pl.halves + head + tail;
+      const int quarters = 4 * (pl.mt * ntb - pl.big), mts = pl.halves;
       int pos = gg_pos(blockIdx.x, quarters + mts * nts);
       if (pos < 0) return;
       if (pos < quarters) {
@@ -507,23 +517,16 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
         n0 = 128 * ni;
         int64_t lo, hi;
         int in;
-        if (mi < pl.halves) {
-          if (!gr.find(mi, [](int64_t x) { return (int)((x % 256 + 127) / 128); }, e, lo, hi, in)) return;
-          m0 = lo + (hi - lo) / 256 * 256 + 128 * in;
-          mrows = (int)(hi - m0 < 128 ? hi - m0 : 128);
-        } else {
-          if (!gr.find_rest(mi - pl.halves, 128, lo, hi)) return;
-          e = -1;
-          m0 = lo;
-          mrows = (int)(hi - lo);
-        }
+        if (!gr.find(mi, [](int64_t x) { return (int)((x % 256 + 127) / 128); }, e, lo, hi, in)) return;
+        m0 = lo + (hi - lo) / 256 * 256 + 128 * in;
+        mrows = (int)(hi - m0 < 128 ? hi - m0 : 128);
       }
     }
     e = __builtin_amdgcn_readfirstlane(e);
     m0 = __builtin_amdgcn_readfirstlane((int)m0);
     n0 = __builtin_amdgcn_readfirstlane(n0);
     mrows = __builtin_amdgcn_readfirstlane(mrows);
-    red = e < 0 ? 0 : (OP == kLinear ? a.K : a.N);
+    red = OP == kLinear ? a.K : a.N;
   }
   const int ncols = cols - n0 < BN ? cols - n0 : BN;
 
@@ -541,7 +544,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
       int64_t row = r;
       bool ok = r < mrows;
       if (gather) {
-        row = ok && e >= 0 ? a.rows[m0 + r] : 0;
+        row = ok ? a.rows[m0 + r] : 0;
         ok = ok && row >= 0 && row < a.T;
       }
       oa.vo[j] = ok ? (uint32_t)((row * a.lda + c) * 2) : kGgOob;
@@ -742,7 +745,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
     }
   } else {
     if constexpr (OP == kLinear) {
-      if (e >= 0 && a.bias) {
+      if (a.bias) {
 #pragma unroll
         for (int y = 0; y < YF; ++y) {
           const int n = wn + 16 * y + 4 * g;
@@ -765,7 +768,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
       }
     }
     uint16_t* out = static_cast<uint16_t*>(a.out);
-    const uint16_t* mk = OP == kDgrad && e >= 0 ? static_cast<const uint16_t*>(a.mask) : nullptr;
+    const uint16_t* mk = OP == kDgrad ? static_cast<const uint16_t*>(a.mask) : nullptr;
 #pragma unroll
     for (int x = 0; x < XF; ++x) {
       const int m = 16 * (2 * x + wr) + i;
@@ -1288,9 +1291,9 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
     big = keep < 0 ? 0 : (a.S / 256 + some) * ntb;
     // quarters, halves of the groups' last rows, rows in no group
     const int64_t quarters = keep < 0 ? a.S / 256 * ntb : kGgCus;
-    small = 4 * quarters + 2 * some * nts + (a.zero_rest ? (a.S / 128 + 2) * nts : 0);
-    const int64_t most = (a.S / 128 + 2 * some + 2) * 2 * ntb;
-    small = small < most ? small : most;
+    small = 4 * quarters + 2 * some * nts;
+    const int64_t most = (a.S / 128 + 2 * some) * 2 * ntb;
+    small = ((small < most ? small : most) + 7) / 8 * 8 + (a.zero_rest ? kGgZero : 0);
   }
   big = (big + 7) / 8 * 8;
   small = (small + 7) / 8 * 8;
@@ -1340,11 +1343,6 @@ hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
 }
 
 }  // namespace
-
-int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a) {
-  (void)op; (void)a;
-  return 0;
-}
 
 hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
   if (a.E < 1 || a.N < 1 || a.K < 1 || a.S < 0 || a.T < 0 || a.S > 0x7fffffffLL || a.T > 0x7fffffffLL ||
