@@ -93,7 +93,15 @@ Span span_of(const torch::Tensor& t) {
 }
 bool meets(const torch::Tensor& a, const torch::Tensor& b) {
   const Span x = span_of(a), y = span_of(b);
-  return x.lo < y.hi && y.lo < x.hi;
+  if (x.lo >= y.hi || y.lo >= x.hi) return false;
+  // column ranges of one buffer lie apart though their spans do not
+  if (a.dim() != 2 || b.dim() != 2) return true;
+  const int64_t ea = a.element_size(), eb = b.element_size();
+  const int64_t ld = a.size(0) > 1 ? a.stride(0) * ea : b.stride(0) * eb;
+  if (ld <= 0 || (b.size(0) > 1 && b.stride(0) * eb != ld)) return true;
+  const int64_t wa = a.size(1) * ea, wb = b.size(1) * eb;
+  const int64_t at = ((y.lo - x.lo) % ld + ld) % ld;  // b's first column, from a's
+  return at < wa || at + wb > ld;
 }
 void check_apart(const torch::Tensor& out, std::initializer_list<const torch::Tensor*> ins, const char* name) {
   for (const torch::Tensor* t : ins) TORCH_CHECK(!t || !meets(out, *t), name, " must not overlap an input");
@@ -363,6 +371,7 @@ torch::Tensor py_grad_norm(const std::vector<torch::Tensor>& grads, bool clip, d
                            const c10::optional<std::vector<torch::Tensor>>& out) {
   TORCH_CHECK(!grads.empty(), "no gradients given");
   TORCH_CHECK(!clip || max_norm >= 0.0, "max_norm must not be negative, got ", max_norm);
+  TORCH_CHECK(!clip || eps >= 0.0, "eps must not be negative, got ", eps);
   const int32_t dt = float_type(grads[0], "gradients");
   TORCH_CHECK(!out || out->size() == grads.size(), "out must hold one tensor a gradient");
   std::vector<ClipTensor> t(grads.size());

@@ -8,6 +8,8 @@
 
 namespace dsml {
 
+constexpr int64_t kMaxThreads = 0xffffffffLL;  // of a launch, along one axis
+
 // ---- router -------------------------------------------------------------
 constexpr int kRouteMaxExperts = 512;
 constexpr int kRouteMaxK = 16;

@@ -180,7 +180,7 @@ template <int DT, bool VEC, int LPR>
 hipError_t launch_combine(const CombineArgs& a, hipStream_t s) {
   const int per = kCbThreads / LPR, chunks = (a.N + 8 * LPR - 1) / (8 * LPR);
   const int64_t blocks = (a.T + per - 1) / per * chunks;
-  if (blocks > 0x7fffffffLL) return hipErrorInvalidValue;
+  if (blocks * kCbThreads > kMaxThreads) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
   if (a.k == 1) hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 1>), grid, dim3(kCbThreads), 0, s, a, chunks);
   else if (a.k == 2) hipLaunchKernelGGL((combine_k<DT, VEC, LPR, 2>), grid, dim3(kCbThreads), 0, s, a, chunks);
@@ -190,7 +190,9 @@ hipError_t launch_combine(const CombineArgs& a, hipStream_t s) {
 template <int DT, bool VEC, int LPR>
 hipError_t launch_combine_bwd(const CombineBwdArgs& a, hipStream_t s) {
   const int per = kCbThreads / LPR;
-  const dim3 grid((uint32_t)((a.T + per - 1) / per));
+  const int64_t blocks = (a.T + per - 1) / per;
+  if (blocks * kCbThreads > kMaxThreads) return hipErrorInvalidValue;
+  const dim3 grid((uint32_t)blocks);
   if (a.k == 1) hipLaunchKernelGGL((combine_bwd_k<DT, VEC, LPR, 1>), grid, dim3(kCbThreads), 0, s, a);
   else if (a.k == 2) hipLaunchKernelGGL((combine_bwd_k<DT, VEC, LPR, 2>), grid, dim3(kCbThreads), 0, s, a);
   else hipLaunchKernelGGL((combine_bwd_k<DT, VEC, LPR, 4>), grid, dim3(kCbThreads), 0, s, a);

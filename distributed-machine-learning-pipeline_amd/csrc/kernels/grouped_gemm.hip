@@ -94,15 +94,16 @@ struct GgGroups {
     n = count((int64_t)b - a);
     inc = gg_scan64(n);
   }
+  // All tiles, `most` at most: more only if the offsets are no plan.
   template <class Count>
-  __device__ __forceinline__ int total(Count count) const {
-    int t = 0;
+  __device__ __forceinline__ int total(Count count, int64_t most) const {
+    int64_t t = 0;
     for (int e0 = 0; e0 < E; e0 += 64) {
       int a, b, n, inc;
       scan(e0, count, a, b, n, inc);
       t += __builtin_amdgcn_readlane(inc, 63);
     }
-    return t;
+    return (int)(t < most ? t : most);
   }
   // The group that holds tile t, its rows and the tile's number in it.
   template <class Count>
@@ -155,7 +156,7 @@ template <class Pick>
 __device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, int BM, bool zero_rest, Pick pick) {
   const GgGroups gr(off, E, S);
   auto count = [BM](int64_t rows) { return (int)((rows + BM - 1) / BM); };
-  const int total = gr.total(count);
+  const int total = gr.total(count, S / BM + E);
   int head = 0, tail = 0;
   if (zero_rest) gr.rest(head, tail, BM);
   GgTile t{-2, 0, 0};
@@ -183,7 +184,10 @@ typedef short gg_i16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) gg_i16x4* gg_lv4;
 typedef uint32_t gg_u4 __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t kGgOob = 0xfffffff0u;    // past every buffer: reads 0
+// Past every buffer: reads 0, also behind a scalar offset that is past the end by
+// itself (sizes and offsets are multiples of 16, so "size - offset" never wraps
+// into the last 16 bytes).
+constexpr uint32_t kGgOob = 0xfffffff0u;
 constexpr int64_t kGgSpan = 0xffffff00LL;   // bytes a buffer descriptor may span
 
 __device__ __forceinline__ gg_u4 gg_desc(const char* base, int64_t bytes) {
@@ -394,9 +398,9 @@ struct GgPlan {
   int halves;      // 128-row tiles of the rows that fill no 256, when the plan leaves those out
 };
 __device__ __forceinline__ GgPlan gg_plan(const GgGroups& gr, int ntb, int nts, int steps, bool only_small) {
-  const int f = gr.total([](int64_t r) { return (int)(r / 256); });
-  const int p = gr.total([](int64_t r) { return r % 256 ? 1 : 0; });
-  const int h = gr.total([](int64_t r) { return (int)((r % 256 + 127) / 128); });
+  const int f = gr.total([](int64_t r) { return (int)(r / 256); }, gr.S / 256);
+  const int p = gr.total([](int64_t r) { return r % 256 ? 1 : 0; }, gr.E);
+  const int h = gr.total([](int64_t r) { return (int)((r % 256 + 127) / 128); }, 2 * (int64_t)gr.E);
   GgPlan best{f, f, 0, h};
   if (only_small) return best;
   int64_t least = -1;
@@ -1246,7 +1250,7 @@ hipError_t launch_any(const GroupedArgs& a, hipStream_t s) {
   const int64_t nt = ((OP == kLinear ? a.N : a.K) + 127) / 128, some = a.E < a.S ? a.E : a.S;
   const int64_t mt = OP == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
   const int64_t blocks = (mt * nt + 7) / 8 * 8;
-  if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
+  if (blocks * 256 > kMaxThreads) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
   if (a.N < 8 || a.K < 8) hipLaunchKernelGGL((grouped_any_k<DT, OP, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((grouped_any_k<DT, OP, false>), grid, dim3(256), 0, s, a);
@@ -1297,7 +1301,7 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
   }
   big = (big + 7) / 8 * 8;
   small = (small + 7) / 8 * 8;
-  if (big > 0x7fffff00LL || small > 0x7fffff00LL) return hipErrorInvalidValue;
+  if (big * 512 > kMaxThreads || small * 256 > kMaxThreads) return hipErrorInvalidValue;
   if (big)
     hipLaunchKernelGGL((grouped_fast_k<DT, OP, 256, 256, 2, 4, GATHER>), dim3((uint32_t)big), dim3(512), 0, s, a, keep);
   if (small)
@@ -1312,7 +1316,7 @@ hipError_t launch_skinny(const GroupedArgs& a, hipStream_t s) {
   int64_t mt = (a.S + 16 * MX - 1) / (16 * MX) + a.E + (a.zero_rest ? 2 : 0);
   mt = mt < a.S ? mt : a.S;
   const int64_t blocks = (int64_t)(nt + 7) / 8 * 8 * mt;
-  if (blocks > 0x7fffff00LL) return hipErrorInvalidValue;
+  if (blocks * 256 > kMaxThreads) return hipErrorInvalidValue;
   hipLaunchKernelGGL((grouped_skinny_k<DT, OP, MX>), dim3((uint32_t)blocks), dim3(256), 0, s, a, nt);
   return hipGetLastError();
 }

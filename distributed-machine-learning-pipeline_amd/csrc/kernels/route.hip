@@ -414,6 +414,7 @@ hipError_t launch_topk(const RouteArgs& a, int L, int blocks, int tiles, int vec
 template <int DT, int K>
 hipError_t launch_bwd(const RouteBwdArgs& a, int L, int vec, int ovec, hipStream_t s) {
   const int64_t per = 256 / L, blocks = (a.T + per - 1) / per;
+  if (blocks * 256 > kMaxThreads) return hipErrorInvalidValue;
 #define DSML_RT(LL) \
   case LL: hipLaunchKernelGGL((route_bwd_k<DT, LL, K>), dim3((uint32_t)blocks), dim3(256), 0, s, a, vec, ovec); break
   switch (L) {

@@ -16,7 +16,8 @@ experts, each token going through the k experts its router chose.
 A token's choice owns a *slot*; slots are ordered by expert, then by token, and
 expert e owns the slots ``offsets[e] .. offsets[e + 1] - 1``.  The plan lives on
 the GPU: nothing here synchronises or copies to the host, and every call can be
-captured into a graph.  Products take bfloat16 or float16 with fp32 sums; weight
+captured into a graph.  The gradients are the explicit calls above (autograd does
+not record a call's kernels).  Products take bfloat16 or float16 with fp32 sums; weight
 and bias gradients are float32, as the trainers keep them.
 
 GPU tensors go to the HIP kernels (mandatory), host tensors to the same math in
@@ -27,6 +28,7 @@ access outside the operands.
 """
 from __future__ import annotations
 
+from operator import index
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -92,8 +94,8 @@ def route_topk(logits: torch.Tensor, k: int, normalize: str = "topk") -> Route:
     whole row (``"all"``); they are not numbers where a chosen logit is +inf.
     """
     if logits.is_cuda:
-        return Route(*require_native().route_topk(logits, int(k), normalize))
-    return _route_ref(logits, int(k), normalize)
+        return Route(*require_native().route_topk(logits, index(k), normalize))
+    return _route_ref(logits, index(k), normalize)
 
 
 def _check_route(T: int, E: int, k: int, normalize: str) -> None:
@@ -315,8 +317,9 @@ def expert_combine(y: torch.Tensor, route: Route, weighted: bool = True,
         _out2(out, T, y.shape[1], y)
     acc = torch.zeros(T, y.shape[1])
     for j in range(k):
-        v = _take(y, route.slots[:, j])
-        acc += v * gates[:, j:j + 1] if weighted else v
+        v, s = _take(y, route.slots[:, j]), route.slots[:, j:j + 1]
+        g = torch.where((s >= 0) & (s < y.shape[0]), gates[:, j:j + 1], torch.zeros(())) if weighted else 1.0
+        acc += v * g
     if out is None:
         return acc.to(y.dtype)
     out.copy_(acc)

@@ -140,9 +140,13 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float =
     grads = list(grads)
     if grads and grads[0].is_cuda:
         return require_native().grad_norm(grads, True, float(max_norm), float(eps), out)
-    if not max_norm >= 0:
-        raise RuntimeError(f"max_norm must not be negative, got {max_norm}")
+    for value, name in ((max_norm, "max_norm"), (eps, "eps")):
+        if not value >= 0:
+            raise RuntimeError(f"{name} must not be negative, got {value}")
     _check_grads(grads, out)
+    written = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in (grads if out is None else out) if t.numel())
+    if any(a + n > b for (a, n), (b, _) in zip(written, written[1:])):
+        raise RuntimeError("clipped gradients must not overlap")
     norm = _norm_ref(grads)
     coef = torch.clamp(max_norm / (norm + eps), max=1.0).float()
     for g, o in zip(grads, grads if out is None else out):

@@ -143,17 +143,19 @@ def test_route_backward_and_combine_refusals():
 @pytest.mark.parametrize("side", ["host", "native"])
 def test_clip_refusals(side):
     if side == "host":
-        def call(g, m=1.0, out=None):
-            return F.clip_grad_norm_(g, m, out=out)
+        def call(g, m=1.0, out=None, eps=None):
+            return F.clip_grad_norm_(g, m, *([] if eps is None else [eps]), out=out)
     else:
         C = _native()
 
-        def call(g, m=1.0, out=None):
-            return C.grad_norm(g, True, m, 1e-6, out)
+        def call(g, m=1.0, out=None, eps=None):
+            return C.grad_norm(g, True, m, 1e-6 if eps is None else eps, out)
     for args, msg in [(([],), "no gradients"), (([torch.ones(2, dtype=torch.int32)],), "float32, bfloat16"),
                       (([torch.ones(2), torch.ones(2, dtype=BF)],), "one type"),
                       (([torch.ones(4, 4).t()[:2]],), "contiguous"), (([torch.ones(2)], -1.0), "negative"),
                       (([torch.ones(2)], math.nan), "negative"),
+                      (([torch.ones(2)], 1.0, None, -1e-6), "eps must not"),
+                      (([torch.ones(2)], 1.0, None, math.nan), "eps must not"),
                       (([torch.ones(2)], 1.0, []), "one tensor a gradient"),
                       (([torch.ones(2)], 1.0, [torch.ones(3)]), "shapes")]:
         with pytest.raises(RuntimeError, match=msg):
@@ -169,6 +171,38 @@ def test_native_clip_refuses_gradients_that_overlap():
             C.grad_norm(grads, True, 1.0, 1e-6, out)
     with pytest.raises(RuntimeError, match="one GPU"):  # disjoint: only the device is wrong
         C.grad_norm([g[:16], g[16:32]], True, 1.0, 1e-6, [g[:16], g[32:48]])
+
+
+def test_host_clip_refuses_gradients_that_overlap():
+    g = torch.ones(64)
+    for grads in ([g, g], [g[:40], g[32:]]):
+        with pytest.raises(RuntimeError, match="overlap"):
+            F.clip_grad_norm_(grads, 1.0)
+    assert F.clip_grad_norm_([g[:32], g[32:]], 4.0) == 8.0 and torch.all((g - 0.5).abs() < 1e-6)
+
+
+def test_columns_of_one_buffer_are_apart():
+    """Operand and result as column ranges of one buffer: refused only where they meet."""
+    C = _native()
+    buf, w, off = torch.ones(6, 48, dtype=BF), torch.ones(1, 16, 16, dtype=BF), torch.tensor([0, 6], dtype=torch.int32)
+    for x, out in [((0, 16), (16, 32)), ((16, 32), (0, 16)), ((32, 48), (8, 24))]:
+        with pytest.raises(RuntimeError, match="GPU tensors"):  # only the device is wrong
+            C.grouped_linear(buf[:, slice(*x)], w, off, out=buf[:, slice(*out)])
+    for x, out in [((0, 16), (8, 24)), ((16, 32), (1, 17)), ((32, 48), (32, 48))]:
+        with pytest.raises(RuntimeError, match="overlap an input"):
+            C.grouped_linear(buf[:, slice(*x)], w, off, out=buf[:, slice(*out)])
+    with pytest.raises(RuntimeError, match="overlap an input"):  # a row further on
+        C.grouped_linear(buf[:5, :16], w, off[:2], out=buf[1:, 8:24])
+
+
+def test_choices_without_a_slot_count_nothing_whatever_their_gate():
+    y = torch.ones(2, 8, dtype=BF)
+    r = X.Route(torch.tensor([[0.5, math.nan]]), torch.tensor([[0, -1]], dtype=torch.int32),
+                torch.tensor([0, 1], dtype=torch.int32), torch.tensor([0, -1], dtype=torch.int32),
+                torch.tensor([[0, -1]], dtype=torch.int32))
+    assert torch.equal(X.expert_combine(y, r), torch.full((1, 8), 0.5, dtype=BF))
+    with pytest.raises(TypeError):
+        X.route_topk(torch.zeros(2, 4), 1.5)
 
 
 # ---- host math --------------------------------------------------------------------

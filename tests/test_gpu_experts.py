@@ -202,6 +202,55 @@ def test_plans_out_of_range_stay_in_the_buffers(K, N):
     assert dw.abs().max() == 0 and torch.equal(db, X.grouped_wgrad(dz, x, off, safe)[1])
 
 
+@pytest.mark.parametrize("sizes,lead,tail", [([2, 0, 3], 5, 30), ([40, 1], 9, 8), ([300, 40], 3, 9000), ([700, 2500], 300, 0),
+                                             ([0, 0], 0, 700), ([0, 513], 2000, 1)])
+@pytest.mark.parametrize("K,N", [(264, 520), (2056, 256)])
+def test_rows_of_no_group_in_whole_words(sizes, lead, tail, K, N):
+    """Aligned operands (padded row strides): the large-tile and single-token
+    kernels zero the rows of no group in a fresh result and leave a given one's."""
+    g, dt = _gen(13), BF
+    S, off = lead + sum(sizes) + tail, offsets_of(sizes, lead).to(DEV)
+    x, dz = _rand(g, S, K + 8, dt=dt)[:, 8:], _rand(g, S, N + 16, dt=dt)[:, :N]
+    x[:lead], dz[:lead] = torch.nan, torch.nan
+    x[S - tail:], dz[S - tail:] = torch.nan, torch.nan
+    w = _rand(g, len(sizes), N, K, dt=dt, scale=K ** -0.5)
+    used = slice(lead, S - tail)
+    for name, call, ref, mag, red, cols in (
+            ("linear", lambda out=None: X.grouped_linear(x, w, off, out=out), *linear64(x, w, sizes, None, False, lead=lead), K, N),
+            ("dgrad", lambda out=None: X.grouped_dgrad(dz, w, off, out=out), *dgrad64(dz, w, sizes, None, lead=lead), N, K)):
+        torch.full((S, cols), 7.0, dtype=dt, device=DEV)  # what a fresh result may find in its memory
+        fresh = call()
+        close(fresh[used], ref[used], rounded_tol(ref, mag, red, dt)[used])
+        assert (fresh[:lead] == 0).all() and (fresh[S - tail:] == 0).all(), name
+        buf = torch.full((S, cols + 8), 7.0, dtype=dt, device=DEV)
+        call(buf[:, 8:])
+        assert torch.equal(buf[used, 8:], fresh[used]), name
+        assert (buf[:lead] == 7).all() and (buf[S - tail:] == 7).all() and (buf[:, :8] == 7).all(), name
+
+
+def test_columns_of_one_buffer_as_operand_and_result():
+    g, dt = _gen(14), BF
+    sizes = [200, 77]
+    off, w = offsets_of(sizes).to(DEV), _rand(g, 2, 128, 64, dt=dt)
+    buf = _rand(g, 277, 256, dt=dt)
+    want = X.grouped_linear(buf[:, 64:128].clone(), w, off)
+    before = buf.clone()
+    X.grouped_linear(buf[:, 64:128], w, off, out=buf[:, 128:])
+    assert torch.equal(buf[:, 128:], want) and torch.equal(buf[:, :128], before[:, :128])
+
+
+def test_all_tokens_to_one_of_many_experts():
+    """A mean of few rows an expert, all of them in one."""
+    g, dt = _gen(15), BF
+    sizes = [0] * 90 + [700] + [0] * 9
+    off, x, w = offsets_of(sizes).to(DEV), _rand(g, 700, 136, dt=dt), _rand(g, 100, 72, 136, dt=dt, scale=0.1)
+    ref, mag = linear64(x, w, sizes, None, False)
+    close(X.grouped_linear(x, w, off), ref, rounded_tol(ref, mag, 136, dt))
+    dz = _rand(g, 700, 72, dt=dt)
+    ref, mag = dgrad64(dz, w, sizes, None)
+    close(X.grouped_dgrad(dz, w, off), ref, rounded_tol(ref, mag, 72, dt))
+
+
 def test_offsets_past_32_bits():
     """More than 2^31 output elements, and rows of x past 2^32 bytes."""
     S, K, N = 560_000, 4096, 3900
