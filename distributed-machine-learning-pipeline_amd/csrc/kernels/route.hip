@@ -94,6 +94,16 @@ __device__ __forceinline__ float rt_sum(float x) {
   return x;
 }
 template <int L>
+__device__ __forceinline__ uint32_t rt_max_u(uint32_t x) {
+  if constexpr (L >= 2) x = max(x, (uint32_t)dpp_i<kDppQuadXor1>((int)x));
+  if constexpr (L >= 4) x = max(x, (uint32_t)dpp_i<kDppQuadXor2>((int)x));
+  if constexpr (L >= 8) x = max(x, (uint32_t)dpp_i<kDppRowHalfMirror>((int)x));
+  if constexpr (L >= 16) x = max(x, (uint32_t)dpp_i<kDppRowMirror>((int)x));
+  if constexpr (L >= 32) x = max(x, (uint32_t)__shfl_xor((int)x, 16));
+  if constexpr (L >= 64) x = max(x, (uint32_t)__shfl_xor((int)x, 32));
+  return x;
+}
+template <int L>
 __device__ __forceinline__ int rt_min(int x) {
   if constexpr (L >= 2) x = min(x, dpp_i<kDppQuadXor1>(x));
   if constexpr (L >= 4) x = min(x, dpp_i<kDppQuadXor2>(x));
@@ -103,6 +113,56 @@ __device__ __forceinline__ int rt_min(int x) {
   if constexpr (L >= 64) x = min(x, __shfl_xor(x, 32));
   return x;
 }
+
+// A lane's logits that were not chosen yet.  take() finds the token's largest
+// (m; -inf: none left) and its lowest column, and removes it.
+//
+// 16-bit types leave at least 13 low bits of their fp32 form zero: value (its bits
+// in an order that unsigned comparison keeps) and column go into one word, and one
+// maximum finds both.
+template <int DT, int L>
+struct RtRow {
+  uint32_t key[8];  // 0: masked
+  __device__ __forceinline__ RtRow(const float (&v)[8], int c0) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = __float_as_uint(v[i] + 0.f);  // -0 is 0
+      const uint32_t o = u ^ (uint32_t)(((int)u >> 31) | (int)0x80000000);
+      key[i] = v[i] > -INFINITY ? (o & ~0x1fffu) | (uint32_t)(0x1fff - (c0 + i)) : 0u;
+    }
+  }
+  __device__ __forceinline__ void take(int, float& m, int& at) {
+    uint32_t k = key[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) k = max(k, key[i]);
+    k = rt_max_u<L>(k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) key[i] = key[i] == k ? 0u : key[i];
+    at = 0x1fff - (int)(k & 0x1fffu);
+    const uint32_t u = k >> 31 ? (k & 0x7fffe000u) : ~(k | 0x1fffu);
+    m = k ? __uint_as_float(u) : -INFINITY;
+  }
+};
+template <int L>
+struct RtRow<kF32, L> {
+  float v[8];
+  __device__ __forceinline__ RtRow(const float (&x)[8], int) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i];
+  }
+  __device__ __forceinline__ void take(int c0, float& m, int& at) {
+    m = v[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, v[i]);
+    m = rt_max<L>(m);
+    at = 0x7fffffff;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) at = v[i] == m ? c0 + i : at;
+    at = rt_min<L>(at);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i == at ? -INFINITY : v[i];
+  }
+};
 
 // Slots of the experts' first choices: exclusive sums of cnt[E] into base[E + 1]
 // (and offsets, by the block that writes them).  One wave.
@@ -181,49 +241,51 @@ __global__ __launch_bounds__(kRtThreads) void route_topk_k(RouteArgs a, int tile
         const int tl = (p0 + q) * kPer + tid / L;
         if (tl >= nt) continue;  // whole L-lane groups leave together
         const int64_t t = t0 + tl;
-        float m = v[q][0];
+        // lane j % L keeps choice j: one exponential, one division, one store each
+        constexpr int KM = (kRouteMaxK + L - 1) / L;
+        float mine[KM], num[KM], top = -INFINITY, sum = 0.f;
+        int pk[KM];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) m = fmaxf(m, v[q][i]);
-        m = rt_max<L>(m);
-        const float top = m;
-        float all = 0.f;
-        if (a.all && top > -INFINITY) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) all += expf(v[q][i] - top);
-          all = rt_sum<L>(all);
+        for (int i = 0; i < KM; ++i) {
+          mine[i] = 0.f;
+          pk[i] = -1;
         }
-        float den = 0.f;
-        float num[kRouteMaxK];
-        int pk[kRouteMaxK];
+        RtRow<DT, L> left(v[q], c0);
 #pragma unroll
         for (int j = 0; j < kRouteMaxK; ++j) {
           if (j >= a.k) break;
-          if (j) {
-            m = v[q][0];
-#pragma unroll
-            for (int i = 1; i < 8; ++i) m = fmaxf(m, v[q][i]);
-            m = rt_max<L>(m);
-          }
-          int at = 0x7fffffff;
-#pragma unroll
-          for (int i = 7; i >= 0; --i) at = v[q][i] == m ? c0 + i : at;
-          at = rt_min<L>(at);
-          const bool live = m > -INFINITY;
-          pk[j] = live ? at : -1;
-          num[j] = live ? expf(m - top) : 0.f;
-          den += num[j];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[q][i] = c0 + i == at ? -INFINITY : v[q][i];
-        }
-        const float d = a.all ? all : den;
-#pragma unroll
-        for (int j = 0; j < kRouteMaxK; ++j) {
-          if (j >= a.k) break;
+          float m;
+          int at;
+          left.take(c0, m, at);
+          if (j == 0) top = m;
           if (sub == j % L) {
-            a.experts[t * a.k + j] = pk[j];
-            a.gates[t * a.k + j] = pk[j] >= 0 ? num[j] / d : 0.f;
-            pick[tl * a.k + j] = pk[j];
-            if (pk[j] >= 0) atomicOr(&mask[pk[j] * 8 + (tl >> 5)], 1u << (tl & 31));
+            mine[j / L] = m;
+            pk[j / L] = m > -INFINITY ? at : -1;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < KM; ++i) {
+          if (L * i >= a.k) break;
+          num[i] = pk[i] >= 0 ? expf(mine[i] - top) : 0.f;
+          sum += num[i];
+        }
+        if (a.all) {
+          sum = 0.f;
+          if (top > -INFINITY) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum += expf(v[q][i] - top);
+          }
+        }
+        sum = rt_sum<L>(sum);
+#pragma unroll
+        for (int i = 0; i < KM; ++i) {
+          if (L * i >= a.k) break;
+          const int j = sub + L * i;
+          if (j < a.k) {
+            a.experts[t * a.k + j] = pk[i];
+            a.gates[t * a.k + j] = pk[i] >= 0 ? num[i] / sum : 0.f;
+            pick[tl * a.k + j] = pk[i];
+            if (pk[i] >= 0) atomicOr(&mask[pk[i] * 8 + (tl >> 5)], 1u << (tl & 31));
           }
         }
       }
