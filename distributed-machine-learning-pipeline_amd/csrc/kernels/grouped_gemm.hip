@@ -1338,11 +1338,17 @@ hipError_t launch_any_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
 template <int DT>
 hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
   if (op == kWgrad) return a.rows ? launch_fast<DT, kWgrad, true>(a, s) : launch_fast<DT, kWgrad>(a, s);
-  // single tokens: by the mean rows of an expert
-  const int64_t mean = a.S / a.E;
-  const int red = op == kLinear ? a.K : a.N;
-  if (mean <= 16) return launch_skinny_op<DT>(op, a, 1, s);
-  if (mean <= 32 && red >= 2048) return launch_skinny_op<DT>(op, a, 2, s);
+  // Few rows.  The kernel that shares the reduction among its waves wins where the
+  // 128 x 128 tiles are fewer than the CUs, each of them a long chain of steps (8
+  // experts of 1024 x 4096, microseconds, 128 x 128 after the slash: 32 rows an
+  // expert 16 / 36, 96 29 / 38, 128 40 / 39; of 1024 x 1024: 32 6 / 12, 96 11 / 13,
+  // 128 15 / 14), that is while its workgroups fit the chip about once, two a CU.
+  // With 16 rows a tile while experts have no more (4096 x 4096: 8 rows 44 / 52, 16
+  // 46 / 55; backward 45 / 42 and 52 / 47), else 32 (24 rows: 47 against 50, and 55).
+  const int red = op == kLinear ? a.K : a.N, cols = op == kLinear ? a.N : a.K;
+  const int64_t wgs = (a.S / 32 + (a.E + 1) / 2) * ((cols + 63) / 64);
+  if (a.S / a.E <= 16) return launch_skinny_op<DT>(op, a, 1, s);
+  if (wgs <= (red >= 2048 ? 640 : 512)) return launch_skinny_op<DT>(op, a, 2, s);
   return op == kLinear ? launch_fast<DT, kLinear>(a, s) : launch_fast<DT, kDgrad>(a, s);
 }
 
