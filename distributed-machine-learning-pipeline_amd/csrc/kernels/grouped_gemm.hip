@@ -5,6 +5,10 @@
 //   dgrad  : dx[s][k]  = (sum_n dz[s][n] w[e][n][k]) * (mask[s][k] > 0)
 //   wgrad  : dw[e][n][k] = sum_s dz[s][n] x[row(s)][k]   (fp32),  db[e][n] = sum_s dz[s][n]
 //
+// Three kernels: grouped_fast_k (operands of whole 16-B words, by LDS-DMA; 256 x 256
+// and 128 x 128 tiles), grouped_skinny_k (few rows: the waves of a workgroup share
+// the reduction) and grouped_any_k (any width, stride and alignment).
+//
 // The offsets live on the GPU (the router writes them), so the host sizes the
 // grid by what they can be at most -- ceil(S / BM) + E row tiles -- and every
 // workgroup finds its expert by a wave scan over the groups' tile counts.
@@ -177,7 +181,15 @@ __device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, 
 // ---------------------------------------------------------------------------
 // Fast path: widths and row strides of whole 16-B words.  256 x 256 output
 // tile, 64-deep steps, 8 waves of 128 x 64 (16x16x32 MFMA), operands by LDS-DMA
-// into two buffers.
+// into a ring of five 32-KiB units: all 160 KiB of LDS, one workgroup a CU.  The
+// 128 x 128 tile (4 waves of 64 x 64, five units of 16 KiB, two workgroups a CU)
+// has the same loop.
+//
+// bf16, 8 experts: 32768 rows x 4096 x 4096 851 us (1292 TFLOP/s; 1535 for a plain
+// library product of that size), the input gradient of 16384 rows 493 (1115), the
+// weight gradient 493 (1116).  With random data the matrix units run at the power
+// limit (788 us of a step count alike on zeros); outside of the products a tile
+// costs about 9 us, of which 4 are its stores and 2 its search and first loads.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* gg_lptr;
 typedef short gg_i16x4 __attribute__((ext_vector_type(4)));
@@ -388,7 +400,9 @@ __device__ __forceinline__ void gg_order(int pos, int mt, int nt, int& mi, int& 
 // as 190; a round that is not full costs a whole one.  So the last round, and the
 // groups' last rows that fill no 256, go where they are done sooner.
 constexpr int kGgCus = 256, kGgRound = 540, kGgSmallMin = 190, kGgGap = 1300;
-// (a second launch costs about 4 us: kGgGap tiles at one step each)
+// (a second launch costs about 4 us: kGgGap tiles at one step each.  Measured with
+// the plan against whole rounds of 256 x 256: 4096 rows, 8 experts of 4096 x 4096,
+// 183 us against 224; 5003 rows, 16 experts of 1000 x 784, 20.5 against 23.8)
 __host__ __device__ __forceinline__ int64_t gg_small_cost(int64_t tiles, int steps) {
   return tiles == 0 ? 0 : (tiles > kGgSmallMin ? tiles : kGgSmallMin) + kGgGap / (steps > 0 ? steps : 1);
 }
@@ -439,6 +453,26 @@ __device__ __forceinline__ bool gg_rows(const GgGroups& gr, const GgPlan& pl, in
   return true;
 }
 
+// wgrad: the rows of group e, or (split) part `part` of them: whole 64-row steps,
+// the first parts full.  A part's sums go to the workspace, [parts][E][N][K] and
+// [parts][E][N].
+__device__ __forceinline__ void gg_part(GroupedArgs& a, int e, int part, int64_t& red0, int& red) {
+  const int64_t lo = gg_clamp(a.offsets[e], 0, a.S), hi = gg_clamp(a.offsets[e + 1], lo, a.S);
+  red0 = lo;
+  red = (int)(hi - lo);
+  if (a.split > 1) {
+    const int64_t rows = ((int64_t)red + 64 * a.split - 1) / (64 * a.split) * 64;
+    red0 = lo + part * rows < hi ? lo + part * rows : hi;
+    red = (int)(hi - red0 < rows ? hi - red0 : rows);
+    a.stro = (int64_t)a.N * a.K;
+    a.ldo = a.K;
+    a.out = a.ws + part * a.E * a.stro;
+    if (a.db) a.db = a.ws + a.split * a.E * a.stro + (int64_t)part * a.E * a.N;
+  }
+  red0 = __builtin_amdgcn_readfirstlane((int)red0);
+  red = __builtin_amdgcn_readfirstlane(red);
+}
+
 // BM x BN tile, WM x WN waves.
 template <int DT, int OP, int BM, int BN, int WM, int WN, bool GATHER>
 __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a, int big) {
@@ -466,10 +500,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
   int sub_m = 0, sub_n = 0;  // kSmall: 128-row (column) half of the tile
   if constexpr (OP == kWgrad) {
     const int mtb = (a.N + 255) / 256, per = mtb * ntb;
-    int pos;
+    int pos, part = 0;
     if constexpr (kSmall) {
-      pos = gg_pos(blockIdx.x, 4 * (per * a.E - big));
+      const int tiles = 4 * (per * a.E - big);
+      pos = gg_pos(blockIdx.x, tiles * a.split);
       if (pos < 0) return;
+      part = pos / tiles;
+      pos -= part * tiles;
       sub_m = (pos >> 1) & 1;
       sub_n = pos & 1;
       pos = big + (pos >> 2);
@@ -484,8 +521,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
     n0 = ni * 256 + 128 * sub_n;
     if (m0 >= a.N || n0 >= cols) return;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
-    red0 = __builtin_amdgcn_readfirstlane((int)gg_clamp(a.offsets[e], 0, a.S));
-    red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
+    gg_part(a, e, part, red0, red);
   } else {
     const GgGroups gr(a.offsets, a.E, a.S);
     if (kSmall && a.zero_rest && blockIdx.x >= gridDim.x - kGgZero) {
@@ -810,7 +846,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
 // take the 64-deep steps in turn, each with a ring of its own (2 slots of 64
 // weight rows and 16 MX operand rows), so the loop has no barrier and 4 x 2 slots
 // a workgroup, two workgroups a CU, are in flight.  The waves' partial tiles are
-// summed in wave order through LDS.
+// summed in wave order through LDS.  16 rows, 8 experts of 4096 x 4096: 54 us with
+// cold weights (4.9 TB/s), 92 with 128 x 128 tiles.
 // ---------------------------------------------------------------------------
 template <int DT, int OP, int MX>
 __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt) {
@@ -977,7 +1014,10 @@ __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt
 // Any width, stride and alignment (rows of odd length start at any 2 bytes, so
 // nothing can go straight to LDS): 128 x 128 tile, 4 waves of 64 x 64, the same
 // LDS images; a thread loads 16-B chunks of a step into registers while the
-// step before is multiplied, and stores them into the other buffer after.
+// step before is multiplied, and stores them into the other buffer after.  On
+// operands that the fast path takes too it needs 51 us against 37 (8192 rows, 8
+// experts of 1000 x 1000) and 1415 against 980 (32768 of 4096 x 4096); 8192 rows of
+// 1003 x 1001: 58.
 // ---------------------------------------------------------------------------
 // Loads are never under a condition (the compiler waits for such a load at the
 // end of its branch: 115 us against 58 at 8192 rows, 8 experts of 1003 x 1001):
@@ -1027,15 +1067,17 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   int e, mrows, red, ni = 0;
   int64_t m0, red0 = 0;
   if constexpr (OP == kWgrad) {
-    const int mtb = (a.N + BM - 1) / BM, per = mtb * nt, pos = gg_pos(blockIdx.x, per * a.E);
+    const int mtb = (a.N + BM - 1) / BM, per = mtb * nt;
+    int pos = gg_pos(blockIdx.x, per * a.E * a.split);
     if (pos < 0) return;
+    const int part = pos / (per * a.E);
+    pos -= part * per * a.E;
     e = pos / per;
     int mi;
     gg_order(pos - e * per, mtb, nt, mi, ni);
     m0 = (int64_t)mi * BM;
     mrows = (int)(a.N - m0 < BM ? a.N - m0 : BM);
-    red0 = __builtin_amdgcn_readfirstlane((int)gg_clamp(a.offsets[e], 0, a.S));
-    red = __builtin_amdgcn_readfirstlane((int)(gg_clamp(a.offsets[e + 1], red0, a.S) - red0));
+    gg_part(a, e, part, red0, red);
   } else {
     const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
       const int pos = gg_pos(blockIdx.x, mts * nt);
@@ -1245,10 +1287,49 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   }
 }
 
+// The parts' sums, in order: 4 columns a thread (V), or 1.
+template <bool V>
+__global__ __launch_bounds__(256) void grouped_join_k(GroupedArgs a) {
+  const int64_t n = (int64_t)a.E * a.N * a.K, nb = a.db ? (int64_t)a.E * a.N : 0, step = (int64_t)gridDim.x * 256;
+  constexpr int W = V ? 4 : 1;
+  const float* bias = a.ws + a.split * n;
+  for (int64_t t = blockIdx.x * 256 + threadIdx.x; t * W < n; t += step) {
+    const int64_t i = t * W, row = i / a.K, c = i - row * a.K, e = row / a.N;
+    float v[W];
+#pragma unroll
+    for (int q = 0; q < W; ++q) v[q] = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < a.split; ++p) {
+      float u[W];
+      if constexpr (V) __builtin_memcpy(u, __builtin_assume_aligned(a.ws + p * n + i, 16), 16);
+      else u[0] = a.ws[p * n + i];
+#pragma unroll
+      for (int q = 0; q < W; ++q) v[q] += u[q];
+    }
+    float* o = static_cast<float*>(a.out) + e * a.stro + (row - e * a.N) * a.ldo + c;
+#pragma unroll
+    for (int q = 0; q < W; ++q) o[q] = v[q];
+  }
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < nb; i += step) {
+    float v = 0.f;
+#pragma unroll 8
+    for (int p = 0; p < a.split; ++p) v += bias[p * nb + i];
+    a.db[i] = v;
+  }
+}
+hipError_t launch_join(const GroupedArgs& a, hipStream_t s) {
+  const bool v = a.K % 4 == 0 && (reinterpret_cast<uintptr_t>(a.ws) & 15) == 0;
+  const int64_t threads = (int64_t)a.E * a.N * a.K / (v ? 4 : 1), blocks = (threads + 255) / 256;
+  const dim3 grid((uint32_t)(blocks < 2048 ? blocks : 2048));
+  if (v) hipLaunchKernelGGL((grouped_join_k<true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((grouped_join_k<false>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
 template <int DT, int OP>
 hipError_t launch_any(const GroupedArgs& a, hipStream_t s) {
   const int64_t nt = ((OP == kLinear ? a.N : a.K) + 127) / 128, some = a.E < a.S ? a.E : a.S;
-  const int64_t mt = OP == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
+  const int64_t mt = OP == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) * a.split : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
   const int64_t blocks = (mt * nt + 7) / 8 * 8;
   if (blocks * 256 > kMaxThreads) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
@@ -1286,8 +1367,9 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
     if (all > 0x3fffffffLL) return hipErrorInvalidValue;
     const int64_t last = all % kGgCus;  // a last round in quarters where that is sooner
     keep = (int)(gg_small_cost(4 * last, (int)(a.S / a.E / 64)) < kGgRound ? all - last : all);
+    if (a.split > 1) keep = 0;
     big = keep;
-    small = 4 * (all - keep);
+    small = 4 * (all - keep) * a.split;
   } else {
     // too few tiles for a round of 256 x 256, if half the groups end inside one
     const int64_t some = a.E < a.S ? a.E : a.S;
@@ -1354,13 +1436,47 @@ hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
 
 }  // namespace
 
-hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
+// Parts of every group's rows in a weight gradient.  A step of 64 rows takes about
+// 0.57 us (1.4 in the kernel for any width), as long as a CU has one 128 x 128 tile;
+// parts shorten that chain and cost their sums' way through the workspace and a
+// launch.  Microseconds without parts and with the number taken here: 20000 rows of
+// 304 x 200 178 / 18 (32), of 301 x 201 437 / 26 (32); 32768 of 1024 x 1024 293 / 95
+// (8); 8 experts, 32768 of 128 x 784 53 / 31 (4).
+int wgrad_parts(const GroupedArgs& a) {
+  const int64_t tiles = (int64_t)a.E * ((a.N + 127) / 128) * ((a.K + 127) / 128), steps = (a.S / a.E + 63) / 64;
+  if (tiles > kGgCus) return 1;
+  const int64_t bytes = (int64_t)a.E * a.N * a.K * 4, step = fast_ok(kWgrad, a) ? 570 : 1400;  // step: ns
+  int best = 1;
+  int64_t least = -1;
+  for (int p = 1; p <= 32; p *= 2) {
+    const int64_t on_cu = (tiles * p + kGgCus - 1) / kGgCus;
+    const int64_t chain = (steps + p - 1) / p * step * (on_cu > 1 ? 85 * on_cu : 100) / 100;
+    const int64_t cost = chain + (p > 1 ? 5000 + (2 * p + 1) * bytes / 4000 : 0);  // 4 TB/s
+    if (least < 0 || cost < least) {
+      least = cost;
+      best = p;
+    }
+  }
+  return best;
+}
+
+int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a) {
+  const int parts = op == kWgrad ? wgrad_parts(a) : 1;
+  return parts > 1 ? (int64_t)parts * a.E * a.N * (a.K + (a.db ? 1 : 0)) : 0;
+}
+
+hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& args, hipStream_t s) {
+  GroupedArgs a = args;
   if (a.E < 1 || a.N < 1 || a.K < 1 || a.S < 0 || a.T < 0 || a.S > 0x7fffffffLL || a.T > 0x7fffffffLL ||
       (a.dtype != kBF16 && a.dtype != kF16))
     return hipErrorInvalidValue;
   if (op != kWgrad && a.S == 0) return hipSuccess;
-  if (fast_ok(op, a)) return a.dtype == kBF16 ? launch_fast_op<kBF16>(op, a, s) : launch_fast_op<kF16>(op, a, s);
-  return a.dtype == kBF16 ? launch_any_op<kBF16>(op, a, s) : launch_any_op<kF16>(op, a, s);
+  a.split = op == kWgrad ? wgrad_parts(a) : 1;
+  if (a.split > 1 && !a.ws) return hipErrorInvalidValue;
+  const hipError_t e = fast_ok(op, a)
+                           ? (a.dtype == kBF16 ? launch_fast_op<kBF16>(op, a, s) : launch_fast_op<kF16>(op, a, s))
+                           : (a.dtype == kBF16 ? launch_any_op<kBF16>(op, a, s) : launch_any_op<kF16>(op, a, s));
+  return e == hipSuccess && a.split > 1 ? launch_join(a, s) : e;
 }
 
 }  // namespace dsml

@@ -18,6 +18,12 @@
 // Block b owns `tiles` consecutive 256-token tiles (at most 256 blocks, so the
 // count table stays small); with one block it finishes alone, else a second
 // launch adds what the blocks before counted.
+//
+// 65536 tokens, 64 experts, k = 4, bf16: 13.8 us (12.6 MB: 2.7 us at the rate of a
+// copy): 9.1 in the first kernel, half of them instructions of the selection, 4.7 in
+// the second, two waits for memory and a launch.  4 tokens: 3.7 us on the GPU; the
+// host needs 6.8 to call.  The gradient of 32768 tokens, 128 experts, k = 8: 9.4 us
+// (3.9 TB/s).
 #include "common.h"
 #include "../dsml.h"
 #include "../experts.h"

@@ -251,6 +251,55 @@ def test_all_tokens_to_one_of_many_experts():
     close(X.grouped_dgrad(dz, w, off), ref, rounded_tol(ref, mag, 72, dt))
 
 
+@pytest.mark.parametrize("sizes,K,N", [([6000], 304, 200), ([3000, 0, 2501], 264, 136), ([5001], 33, 70), ([20000], 8, 8),
+                                       ([4000, 1, 130], 512, 384), ([9000, 64], 5, 3)])
+@pytest.mark.parametrize("dt", [BF, FP])
+@pytest.mark.parametrize("gather", [False, True])
+def test_wgrad_of_few_tiles_and_many_rows(sizes, K, N, dt, gather):
+    """Groups whose rows are summed in parts: the same bound, the same bits every
+    time, given buffers written in place and nothing around them."""
+    g = _gen(sum(sizes) + K)
+    lead, tail, E = 7, 33, len(sizes)
+    S = lead + sum(sizes) + tail
+    off = offsets_of(sizes, lead).to(DEV)
+    T = 500 if gather else S
+    x, dz = _rand(g, T, K, dt=dt), _rand(g, S, N, dt=dt, scale=0.1)
+    dz[:lead], dz[S - tail:] = torch.nan, torch.nan
+    rows = _rows(g, S, T) if gather else None
+    dw, dwm, db, dbm = wgrad64(dz, x, sizes, rows, lead=lead)
+    got, gb = X.grouped_wgrad(dz, x, off, rows)
+    close(got, dw, rounded_tol(dw, dwm, max(sizes), torch.float32))
+    close(gb, db, rounded_tol(db, dbm, max(sizes), torch.float32))
+    buf, bb = torch.full((E, N + 1, K + 4), 7.0, device=DEV), torch.full((E, N), 7.0, device=DEV)
+    X.grouped_wgrad(dz, x, off, rows, dw=buf[:, :N, 4:], db=bb)
+    close(buf[:, :N, 4:], dw, rounded_tol(dw, dwm, max(sizes), torch.float32))
+    assert (buf[:, N] == 7).all() and (buf[:, :, :4] == 7).all() and torch.equal(bb, gb)
+    again, none = X.grouped_wgrad(dz, x, off, rows, bias=False)
+    assert none is None and torch.equal(again, got)
+
+
+def test_wgrad_in_parts_in_two_graphs():
+    """Each captured call has a workspace of its own; replayed on new values between eager calls."""
+    g = _gen(21)
+    off = offsets_of([3000, 2000]).to(DEV)
+    dz, x = _rand(g, 5000, 72, dt=BF), _rand(g, 5000, 40, dt=BF)
+    X.grouped_wgrad(dz, x, off)
+    graphs, outs = [], []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(X.grouped_wgrad(dz, x, off))
+        graphs.append(gr)
+    for seed in (1, 2, 3):
+        dz.copy_(_rand(_gen(seed), 5000, 72, dt=BF))
+        want = X.grouped_wgrad(dz, x, off)
+        for gr in graphs:
+            gr.replay()
+        torch.cuda.synchronize(DEV)
+        for o in outs:
+            assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
+
+
 def test_offsets_past_32_bits():
     """More than 2^31 output elements, and rows of x past 2^32 bytes."""
     S, K, N = 560_000, 4096, 3900
