@@ -182,4 +182,16 @@ __device__ __forceinline__ void quad_argmax(float& mx, int& amax) {
   }
 }
 
+// 8 16-bit elements without the first s (0..8), zeros behind.
+__device__ __forceinline__ uint4 drop_front8(uint4 v, int s) {
+  uint64_t lo = ((uint64_t)v.y << 32) | v.x, hi = ((uint64_t)v.w << 32) | v.z;
+  const int q = s & 3;
+  lo = s & 4 ? hi : lo;
+  hi = s & 4 ? 0 : hi;
+  lo = q ? (lo >> (16 * q)) | (hi << (64 - 16 * q)) : lo;
+  hi >>= 16 * q;
+  if (s >= 8) lo = hi = 0;
+  return make_uint4((uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32));
+}
+
 }  // namespace dsml

@@ -1017,7 +1017,8 @@ __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt
 // step before is multiplied, and stores them into the other buffer after.  On
 // operands that the fast path takes too it needs 51 us against 37 (8192 rows, 8
 // experts of 1000 x 1000) and 1415 against 980 (32768 of 4096 x 4096); 8192 rows of
-// 1003 x 1001: 58.
+// 1003 x 1001 with a bias: 36 (44 with the bias loaded at its use; backward with a
+// mask 46 and 52).
 // ---------------------------------------------------------------------------
 // Loads are never under a condition (the compiler waits for such a load at the
 // end of its branch: 115 us against 58 at 8192 rows, 8 experts of 1003 x 1001):
@@ -1043,14 +1044,7 @@ __device__ __forceinline__ void gg_load8(GgChunk& u, const uint16_t* row, int c,
   }
 }
 __device__ __forceinline__ gg_u4 gg_settle(const GgChunk& u) {
-  uint64_t lo = ((uint64_t)u.v[1] << 32) | u.v[0], hi = ((uint64_t)u.v[3] << 32) | u.v[2];
-  const int s = u.shift & 3;
-  lo = u.shift & 4 ? hi : lo;
-  hi = u.shift & 4 ? 0 : hi;
-  lo = s ? (lo >> (16 * s)) | (hi << (64 - 16 * s)) : lo;
-  hi >>= 16 * s;
-  if (u.shift >= 8) lo = hi = 0;
-  return gg_u4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+  return __builtin_bit_cast(gg_u4, drop_front8(__builtin_bit_cast(uint4, u.v), u.shift));
 }
 
 template <int DT, int OP, bool NARROW>
@@ -1255,6 +1249,41 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   } else {
     uint16_t* out = static_cast<uint16_t*>(a.out);
     const uint16_t* mk = OP == kDgrad && e >= 0 ? static_cast<const uint16_t*>(a.mask) : nullptr;
+    // bias and mask: all loads first and none under a condition, from the nearest
+    // column (row) that exists
+    f32x4 bias[YF];
+    if (OP == kLinear && e >= 0 && a.bias) {
+#pragma unroll
+      for (int y = 0; y < YF; ++y)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = n0 + wn + 16 * y + 4 * g + q;
+          bias[y][q] = a.bias[(int64_t)e * a.ldbias + (n < cols ? n : cols - 1)];
+        }
+    } else {
+#pragma unroll
+      for (int y = 0; y < YF; ++y) bias[y] = {0.f, 0.f, 0.f, 0.f};
+    }
+    uint64_t keep[XF][YF];  // 4 mask values each
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      const int m = 16 * (2 * x + wr) + i;
+      const uint16_t* row = mk ? mk + (m0 + (m < mrows ? m : mrows - 1)) * a.ldmask : nullptr;
+#pragma unroll
+      for (int y = 0; y < YF; ++y) {
+        const int n = n0 + wn + 16 * y + 4 * g;
+        keep[x][y] = 0;
+        if (mk) {
+          if constexpr (!NARROW) {
+            __builtin_memcpy(&keep[x][y], row + (n < cols - 4 ? n : cols - 4), 8);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (n + q < cols) keep[x][y] |= (uint64_t)row[n + q] << (16 * q);
+          }
+        }
+      }
+    }
 #pragma unroll
     for (int x = 0; x < XF; ++x) {
       const int m = 16 * (2 * x + wr) + i;
@@ -1264,15 +1293,17 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
       for (int y = 0; y < YF; ++y) {
         const int n = wn + 16 * y + 4 * g;
         f32x4 v = acc[x][y];
+        if constexpr (OP == kLinear) {
+          v += bias[y];
+          if (a.relu) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          if (n + q >= ncols) continue;
-          if constexpr (OP == kLinear) {
-            if (e >= 0 && a.bias) v[q] += a.bias[(int64_t)e * a.ldbias + n0 + n + q];
-            if (a.relu) v[q] = v[q] < 0.f ? 0.f : v[q];
-          } else {
-            if (mk && !(gg_f<DT>(mk[(m0 + m) * a.ldmask + n0 + n + q]) > 0.f)) v[q] = 0.f;
+            for (int q = 0; q < 4; ++q) v[q] = v[q] < 0.f ? 0.f : v[q];
           }
+        } else if (mk) {
+          const int past = NARROW ? 0 : n0 + n - (cols - 4);  // columns the load was moved back by
+          const uint64_t k = keep[x][y] >> (past < 1 ? 0 : (past < 4 ? 16 * past : 63));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) v[q] = gg_f<DT>((uint16_t)(k >> (16 * q))) > 0.f ? v[q] : 0.f;
         }
         const uint2 u = make_uint2(gg_pack2<DT>(v[0], v[1]), gg_pack2<DT>(v[2], v[3]));
         if (n + 4 <= ncols) {
@@ -1371,9 +1402,13 @@ hipError_t launch_fast(const GroupedArgs& a, hipStream_t s) {
     big = keep;
     small = 4 * (all - keep) * a.split;
   } else {
-    // too few tiles for a round of 256 x 256, if half the groups end inside one
+    // Too few tiles for a round of 256 x 256, if half the groups end inside one, or a
+    // reduction so short that a tile is mostly its first loads and its stores, which
+    // two workgroups a CU hide from each other (with 256 x 256 / 128 x 128 only: 13424
+    // rows of 568, reduction 1024, 36 / 29 us; 8192 rows of 4096, 256 53 / 41, 512 64 /
+    // 67; 32768 of 4096, 64 104 / 103, 256 146 / 156).
     const int64_t some = a.E < a.S ? a.E : a.S;
-    if (4 * (a.S / 256 + some / 2) * ntb <= kGgRound) keep = -1;
+    if (4 * (a.S / 256 + some / 2) * ntb <= 700 || (OP == kLinear ? a.K : a.N) <= 256) keep = -1;
     big = keep < 0 ? 0 : (a.S / 256 + some) * ntb;
     // quarters, halves of the groups' last rows, rows in no group
     const int64_t quarters = keep < 0 ? a.S / 256 * ntb : kGgCus;
