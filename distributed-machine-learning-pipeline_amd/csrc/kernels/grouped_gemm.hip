@@ -858,13 +858,21 @@ __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int rr = lane >> 3, p = lane & 7, i = lane & 15, g = lane >> 4;
   const int cols = OP == kLinear ? a.N : a.K;
-  // an XCD takes every 8th column tile, all its row tiles together
+  // An XCD takes every 8th column tile, all its row tiles together; with fewer than
+  // 8 columns an eighth of the tiles.  (An eighth each with more: neighbouring rows
+  // of the weights are no longer read at once, 16 rows, 8 experts of 4096 x 4096: 54 us become 65.)
   int ni = 0;
   const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
+    const int x = blockIdx.x & 7, in = blockIdx.x >> 3;
     if (mts == 0) return -1;
-    const int j = blockIdx.x >> 3;
-    ni = (blockIdx.x & 7) + 8 * (j / mts);
-    return ni < nt ? j % mts : -1;
+    if (nt >= 8) {
+      ni = x + 8 * (in / mts);
+      return ni < nt ? in % mts : -1;
+    }
+    const int all = mts * nt, share = (all + 7) >> 3, u = x * share + in;
+    if (in >= share || u >= all) return -1;
+    ni = u / mts;
+    return u - ni * mts;
   });
   if (t.e == -2) return;
   const int e = __builtin_amdgcn_readfirstlane(t.e);
@@ -1432,7 +1440,7 @@ hipError_t launch_skinny(const GroupedArgs& a, hipStream_t s) {
   const int nt = (cols + 63) / 64;
   int64_t mt = (a.S + 16 * MX - 1) / (16 * MX) + a.E + (a.zero_rest ? 2 : 0);
   mt = mt < a.S ? mt : a.S;
-  const int64_t blocks = (int64_t)(nt + 7) / 8 * 8 * mt;
+  const int64_t blocks = nt >= 8 ? (int64_t)(nt + 7) / 8 * 8 * mt : (nt * mt + 7) / 8 * 8;
   if (blocks * 256 > kMaxThreads) return hipErrorInvalidValue;
   hipLaunchKernelGGL((grouped_skinny_k<DT, OP, MX>), dim3((uint32_t)blocks), dim3(256), 0, s, a, nt);
   return hipGetLastError();

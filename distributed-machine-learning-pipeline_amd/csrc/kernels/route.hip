@@ -70,23 +70,37 @@ __device__ __forceinline__ void rt_row(const void* logits, int64_t row, int E, i
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = -INFINITY;
     }
-  } else {
+  } else {  // no load under a condition: a column past the end is read as the last
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < E ? rt_load<DT>(logits, row + c0 + i) : -INFINITY;
+    for (int i = 0; i < 8; ++i) v[i] = rt_load<DT>(logits, row + (c0 + i < E ? c0 + i : E - 1));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i < E ? v[i] : -INFINITY;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = v[i] == v[i] ? v[i] : -INFINITY;
 }
 
 // Reductions over a token's L lanes (every lane gets the result).
+// Across the two rows of 16 lanes of each half (FAR: the two halves) of a wave.
+template <bool FAR, class T, class Op>
+__device__ __forceinline__ T rt_rows(T x, Op op) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  if constexpr (FAR) {
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return op(__builtin_bit_cast(T, (uint32_t)s[0]), __builtin_bit_cast(T, (uint32_t)s[1]));
+  } else {
+    const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return op(__builtin_bit_cast(T, (uint32_t)s[0]), __builtin_bit_cast(T, (uint32_t)s[1]));
+  }
+}
 template <int L>
 __device__ __forceinline__ float rt_max(float x) {
   if constexpr (L >= 2) x = fmaxf(x, dpp_f<kDppQuadXor1>(x));
   if constexpr (L >= 4) x = fmaxf(x, dpp_f<kDppQuadXor2>(x));
   if constexpr (L >= 8) x = fmaxf(x, dpp_f<kDppRowHalfMirror>(x));
   if constexpr (L >= 16) x = fmaxf(x, dpp_f<kDppRowMirror>(x));
-  if constexpr (L >= 32) x = fmaxf(x, __shfl_xor(x, 16));
-  if constexpr (L >= 64) x = fmaxf(x, __shfl_xor(x, 32));
+  if constexpr (L >= 32) x = rt_rows<false>(x, [](float p, float q) { return fmaxf(p, q); });
+  if constexpr (L >= 64) x = rt_rows<true>(x, [](float p, float q) { return fmaxf(p, q); });
   return x;
 }
 template <int L>
@@ -95,8 +109,8 @@ __device__ __forceinline__ float rt_sum(float x) {
   if constexpr (L >= 4) x += dpp_f<kDppQuadXor2>(x);
   if constexpr (L >= 8) x += dpp_f<kDppRowHalfMirror>(x);
   if constexpr (L >= 16) x += dpp_f<kDppRowMirror>(x);
-  if constexpr (L >= 32) x += __shfl_xor(x, 16);
-  if constexpr (L >= 64) x += __shfl_xor(x, 32);
+  if constexpr (L >= 32) x = rt_rows<false>(x, [](float p, float q) { return p + q; });
+  if constexpr (L >= 64) x = rt_rows<true>(x, [](float p, float q) { return p + q; });
   return x;
 }
 template <int L>
@@ -105,8 +119,8 @@ __device__ __forceinline__ uint32_t rt_max_u(uint32_t x) {
   if constexpr (L >= 4) x = max(x, (uint32_t)dpp_i<kDppQuadXor2>((int)x));
   if constexpr (L >= 8) x = max(x, (uint32_t)dpp_i<kDppRowHalfMirror>((int)x));
   if constexpr (L >= 16) x = max(x, (uint32_t)dpp_i<kDppRowMirror>((int)x));
-  if constexpr (L >= 32) x = max(x, (uint32_t)__shfl_xor((int)x, 16));
-  if constexpr (L >= 64) x = max(x, (uint32_t)__shfl_xor((int)x, 32));
+  if constexpr (L >= 32) x = rt_rows<false>(x, [](uint32_t p, uint32_t q) { return max(p, q); });
+  if constexpr (L >= 64) x = rt_rows<true>(x, [](uint32_t p, uint32_t q) { return max(p, q); });
   return x;
 }
 template <int L>
@@ -115,8 +129,8 @@ __device__ __forceinline__ int rt_min(int x) {
   if constexpr (L >= 4) x = min(x, dpp_i<kDppQuadXor2>(x));
   if constexpr (L >= 8) x = min(x, dpp_i<kDppRowHalfMirror>(x));
   if constexpr (L >= 16) x = min(x, dpp_i<kDppRowMirror>(x));
-  if constexpr (L >= 32) x = min(x, __shfl_xor(x, 16));
-  if constexpr (L >= 64) x = min(x, __shfl_xor(x, 32));
+  if constexpr (L >= 32) x = rt_rows<false>(x, [](int p, int q) { return min(p, q); });
+  if constexpr (L >= 64) x = rt_rows<true>(x, [](int p, int q) { return min(p, q); });
   return x;
 }
 

@@ -319,7 +319,7 @@ def test_offsets_past_32_bits():
 
 # ---- router -------------------------------------------------------------------------
 ROUTES = [(1, 1, 1), (4, 8, 2), (1, 13, 3), (64, 16, 16), (255, 30, 5), (256, 64, 4), (257, 64, 4), (1000, 100, 8),
-          (600, 256, 8), (300, 512, 16), (3000, 7, 2)]
+          (600, 256, 8), (300, 512, 16), (3000, 7, 2), (40, 200, 3), (70, 133, 6), (33, 301, 4), (20, 512, 2)]
 
 
 def _logits(T, E, dt, seed):
@@ -375,7 +375,8 @@ def test_route_without_tokens():
 # ---- combine --------------------------------------------------------------------------
 @pytest.mark.parametrize("dt", [BF, FP])
 @pytest.mark.parametrize("T,k,N", [(1, 1, 1), (3, 2, 8), (5, 4, 13), (130, 3, 70), (33, 6, 128), (64, 16, 256),
-                                   (257, 2, 784), (20, 5, 4096), (9, 2, 4100)])
+                                   (257, 2, 784), (20, 5, 4096), (9, 2, 4100),
+                                   (1100, 2, 784), (1030, 5, 1001), (2000, 3, 7), (1025, 1, 519)])
 def test_combine(T, k, N, dt):
     g = _gen(T + N)
     logits = torch.randn(T, max(k, 20), generator=g, device=DEV)
