@@ -59,8 +59,8 @@ struct GroupedArgs {
   int64_t ldmask;
   void* out;  // linear: [S][ldo] (N columns); dgrad: [S][ldo] (K columns); wgrad: fp32 [E][N][K]
   int64_t ldo, stro;
-  float* ws;  // wgrad: grouped_ws_floats() of workspace, if any
-  int split;  // wgrad: parts of every group's rows (set by grouped_gemm)
+  float* ws;  // grouped_ws_floats() of workspace, if any
+  int split;  // parts of the reduction (set by grouped_gemm)
   float* db;  // wgrad: fp32 [E][N], or null
   int64_t S, T;  // slots, rows of x
   int E, N, K;

@@ -189,7 +189,7 @@ __device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, 
 // library product of that size), the input gradient of 16384 rows 493 (1115), the
 // weight gradient 493 (1116).  With random data the matrix units run at the power
 // limit (788 us of a step count alike on zeros); outside of the products a tile
-// costs about 9 us, of which 4 are its stores and 2 its search and first loads.
+// costs about 8 us: its stores, its search, its first loads.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* gg_lptr;
 typedef short gg_i16x4 __attribute__((ext_vector_type(4)));
@@ -1091,13 +1091,13 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   const int cols = OP == kLinear ? a.N : a.K, nt = (cols + BN - 1) / BN;
   const uint16_t* A = static_cast<const uint16_t*>(a.a);
   const uint16_t* B = static_cast<const uint16_t*>(a.b);
-  int e, mrows, red, ni = 0;
+  int e, mrows, red, ni = 0, part = 0;
   int64_t m0, red0 = 0;
   if constexpr (OP == kWgrad) {
     const int mtb = (a.N + BM - 1) / BM, per = mtb * nt;
     int pos = gg_pos(blockIdx.x, per * a.E * a.split);
     if (pos < 0) return;
-    const int part = pos / (per * a.E);
+    part = pos / (per * a.E);
     pos -= part * per * a.E;
     e = pos / per;
     int mi;
@@ -1107,13 +1107,14 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
     gg_part(a, e, part, red0, red);
   } else {
     const GgTile t = gg_find(a.offsets, a.E, a.S, BM, a.zero_rest, [&](int mts) {
-      const int pos = gg_pos(blockIdx.x, mts * nt);
+      const int pos = gg_pos(blockIdx.x, mts * nt * a.split);
       if (pos < 0) return -1;
+      part = pos / (mts * nt);
       int mi;
-      gg_order(pos, mts, nt, mi, ni);
+      gg_order(pos - part * mts * nt, mts, nt, mi, ni);
       return mi;
     });
-    if (t.e == -2) return;
+    if (t.e == -2 || (t.e < 0 && a.split > 1)) return;  // (the join clears rows of no group)
     e = __builtin_amdgcn_readfirstlane(t.e);
     m0 = __builtin_amdgcn_readfirstlane((int)t.s0);
     mrows = __builtin_amdgcn_readfirstlane((int)(t.s1 - t.s0));
@@ -1197,7 +1198,13 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   ra.init(wr, lane);
   rb.init(YF * wc, lane);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(gg_lptr)lds;
-  const int steps = (red + 63) / 64;
+  // steps [first, steps): all, or a part of the reduction
+  int steps = (red + 63) / 64, first = 0;
+  if (OP != kWgrad && a.split > 1) {
+    const int per = (steps + a.split - 1) / a.split;
+    first = part * per < steps ? part * per : steps;
+    steps = steps - first < per ? steps : first + per;
+  }
   // whole chunks need no shifting: full tiles of rows that exist, but a last step
   const bool whole = !NARROW && mrows == BM && ncols == BN && !(OP != kDgrad && a.rows);
   auto store = [&](int t, const Set& u) {
@@ -1231,13 +1238,13 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
   };
   // step t is multiplied while steps t + 1 (stored after it) and t + 2 are in flight
   Set u0, u1;
-  if (steps > 0) {
-    load(0, u0);
-    load(steps > 1 ? 1 : 0, u1);
-    store(0, u0);
-    load(steps > 2 ? 2 : 0, u0);
+  if (steps > first) {
+    load(first, u0);
+    load(steps > first + 1 ? first + 1 : first, u1);
+    store(first, u0);
+    load(steps > first + 2 ? first + 2 : first, u0);
     __syncthreads();
-    for (int t = 0; t < steps; t += 2) {
+    for (int t = first; t < steps; t += 2) {
       multiply(t);
       if (t + 1 < steps) {
         store(t + 1, u1);
@@ -1267,6 +1274,24 @@ __global__ __launch_bounds__(256, 2) void grouped_any_k(GroupedArgs a) {
       const int m = 16 * (2 * x + wr) + i;
       if (m >= mrows) continue;
       float* o = out + (m0 + m) * a.ldo + n0;
+#pragma unroll
+      for (int y = 0; y < YF; ++y) {
+        const int n = wn + 16 * y + 4 * g;
+        if (n + 4 <= ncols) {
+          __builtin_memcpy(o + n, &acc[x][y], 16);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+            if (n + q < ncols) o[n + q] = acc[x][y][q];
+        }
+      }
+    }
+  } else if (a.split > 1) {  // [parts][S][columns]
+#pragma unroll
+    for (int x = 0; x < XF; ++x) {
+      const int m = 16 * (2 * x + wr) + i;
+      if (m >= mrows) continue;
+      float* o = a.ws + ((int64_t)part * a.S + m0 + m) * cols + n0;
 #pragma unroll
       for (int y = 0; y < YF; ++y) {
         const int n = wn + 16 * y + 4 * g;
@@ -1390,15 +1415,72 @@ hipError_t launch_join(const GroupedArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 
+// The same for rows of an output: a wave 256 columns of a row, which it finds the
+// expert of for the bias; rows of no group are cleared or left.
+template <int DT, int OP>
+__global__ __launch_bounds__(256) void grouped_join_rows_k(GroupedArgs a) {
+  const int lane = threadIdx.x & 63, cols = OP == kLinear ? a.N : a.K;
+  const int64_t r = blockIdx.x * 4 + (threadIdx.x >> 6), n = a.S * cols;
+  if (r >= a.S) return;
+  int e = -1;
+  for (int e0 = 0; e0 < a.E && e < 0; e0 += 64) {
+    bool in = false;
+    if (e0 + lane < a.E) {
+      const int64_t lo = gg_clamp(a.offsets[e0 + lane], 0, a.S), hi = gg_clamp(a.offsets[e0 + lane + 1], lo, a.S);
+      in = r >= lo && r < hi;
+    }
+    const unsigned long long hit = __ballot(in);
+    if (hit) e = e0 + __ffsll(hit) - 1;
+  }
+  if (e < 0 && !a.zero_rest) return;
+  const int c0 = 256 * blockIdx.y + lane;  // and c0 + 64, + 128, + 192; past the end: the last column's loads
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (e >= 0) {
+    for (int q0 = 0; q0 < a.split; q0 += 8) {  // 8 parts in flight; past the last: the last's, not added
+      float t[8][4];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const float* p = a.ws + (q0 + q < a.split ? q0 + q : a.split - 1) * n + r * cols;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) t[q][u] = p[c0 + 64 * u < cols ? c0 + 64 * u : cols - 1];
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] += q0 + q < a.split ? t[q][u] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int c = c0 + 64 * u;
+    if (c >= cols) continue;
+    float x = v[u];
+    if (e >= 0) {
+      if constexpr (OP == kLinear) {
+        if (a.bias) x += a.bias[(int64_t)e * a.ldbias + c];
+        if (a.relu) x = x < 0.f ? 0.f : x;
+      } else if (a.mask) {
+        x = gg_f<DT>(static_cast<const uint16_t*>(a.mask)[r * a.ldmask + c]) > 0.f ? x : 0.f;
+      }
+    }
+    static_cast<uint16_t*>(a.out)[r * a.ldo + c] = (uint16_t)gg_pack2<DT>(x, x);
+  }
+}
+
 template <int DT, int OP>
 hipError_t launch_any(const GroupedArgs& a, hipStream_t s) {
   const int64_t nt = ((OP == kLinear ? a.N : a.K) + 127) / 128, some = a.E < a.S ? a.E : a.S;
-  const int64_t mt = OP == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) * a.split : (a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0);
+  const int64_t mt = OP == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) * a.split : ((a.S + 127) / 128 + some + (a.zero_rest ? 2 : 0)) * a.split;
   const int64_t blocks = (mt * nt + 7) / 8 * 8;
   if (blocks * 256 > kMaxThreads) return hipErrorInvalidValue;
   const dim3 grid((uint32_t)blocks);
   if (a.N < 8 || a.K < 8) hipLaunchKernelGGL((grouped_any_k<DT, OP, true>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((grouped_any_k<DT, OP, false>), grid, dim3(256), 0, s, a);
+  if constexpr (OP != kWgrad) {
+    if (a.split > 1)
+      hipLaunchKernelGGL((grouped_join_rows_k<DT, OP>), dim3((uint32_t)((a.S + 3) / 4), (uint32_t)((nt + 1) / 2)), dim3(256),
+                         0, s, a);
+  }
   return hipGetLastError();
 }
 
@@ -1504,21 +1586,31 @@ hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
 
 }  // namespace
 
-// Parts of every group's rows in a weight gradient.  A step of 64 rows takes about
-// 0.57 us (1.4 in the kernel for any width), as long as a CU has one 128 x 128 tile;
-// parts shorten that chain and cost their sums' way through the workspace and a
-// launch.  Microseconds without parts and with the number taken here: 20000 rows of
-// 304 x 200 178 / 18 (32), of 301 x 201 437 / 26 (32); 32768 of 1024 x 1024 293 / 95
-// (8); 8 experts, 32768 of 128 x 784 53 / 31 (4).
-int wgrad_parts(const GroupedArgs& a) {
-  const int64_t tiles = (int64_t)a.E * ((a.N + 127) / 128) * ((a.K + 127) / 128), steps = (a.S / a.E + 63) / 64;
+// Parts of a reduction whose 128 x 128 tiles leave CUs idle: a group's rows (weight
+// gradients), or all of it (the kernel for any width).  A step of 64 takes about
+// 0.57 us (1.4 in the kernel for any width), as long as a CU has one tile; parts
+// shorten that chain and cost their sums' way through the workspace and a launch.
+// Microseconds without parts and with the number taken here: weight gradients of 20000
+// rows of 304 x 200 178 / 18 (32), of 301 x 201 437 / 26 (32), of 32768 of 1024 x 1024
+// 293 / 95 (8), 8 experts, 32768 of 128 x 784 53 / 31 (4); products of 75 rows, 21 experts
+// of 248 x 3154, 59 / 21, backward of 101 rows, 2 experts, 1788 to 159, 44 / 12.
+int parts_of(GroupedOp op, const GroupedArgs& a) {
+  const bool fast = fast_ok(op, a);
+  if (a.S == 0 || (op != kWgrad && fast)) return 1;
+  const int cols = op == kLinear ? a.N : a.K, red = op == kLinear ? a.K : a.N;
+  const int64_t nt = (cols + 127) / 128, some = a.E < a.S ? a.E : a.S;
+  const int64_t tiles = nt * (op == kWgrad ? (int64_t)a.E * ((a.N + 127) / 128) : a.S / 128 + some);
   if (tiles > kGgCus) return 1;
-  const int64_t bytes = (int64_t)a.E * a.N * a.K * 4, step = fast_ok(kWgrad, a) ? 570 : 1400;  // step: ns
+  const int64_t steps = ((op == kWgrad ? a.S / a.E : red) + 63) / 64, step = fast ? 570 : 1400;  // step: ns
+  const int64_t bytes = (op == kWgrad ? (int64_t)a.E * a.N : a.S) * cols * 4;
+  const int64_t weights = op == kWgrad ? 0 : some * a.N * a.K * 2 / 3000;  // ns to read them
   int best = 1;
   int64_t least = -1;
   for (int p = 1; p <= 32; p *= 2) {
     const int64_t on_cu = (tiles * p + kGgCus - 1) / kGgCus;
-    const int64_t chain = (steps + p - 1) / p * step * (on_cu > 1 ? 85 * on_cu : 100) / 100;
+    // two tiles on a CU share its fetch: no gain in the kernel for any width
+    int64_t chain = (steps + p - 1) / p * step * (on_cu > 1 ? (fast ? 85 : 100) * on_cu : 100) / 100;
+    chain = chain > weights ? chain : weights;
     const int64_t cost = chain + (p > 1 ? 5000 + (2 * p + 1) * bytes / 4000 : 0);  // 4 TB/s
     if (least < 0 || cost < least) {
       least = cost;
@@ -1529,8 +1621,10 @@ int wgrad_parts(const GroupedArgs& a) {
 }
 
 int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a) {
-  const int parts = op == kWgrad ? wgrad_parts(a) : 1;
-  return parts > 1 ? (int64_t)parts * a.E * a.N * (a.K + (a.db ? 1 : 0)) : 0;
+  const int parts = parts_of(op, a);
+  if (parts == 1) return 0;
+  if (op == kWgrad) return (int64_t)parts * a.E * a.N * (a.K + (a.db ? 1 : 0));
+  return parts * a.S * (op == kLinear ? a.N : a.K);
 }
 
 hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& args, hipStream_t s) {
@@ -1539,12 +1633,12 @@ hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& args, hipStream_t s) {
       (a.dtype != kBF16 && a.dtype != kF16))
     return hipErrorInvalidValue;
   if (op != kWgrad && a.S == 0) return hipSuccess;
-  a.split = op == kWgrad ? wgrad_parts(a) : 1;
+  a.split = parts_of(op, a);
   if (a.split > 1 && !a.ws) return hipErrorInvalidValue;
   const hipError_t e = fast_ok(op, a)
                            ? (a.dtype == kBF16 ? launch_fast_op<kBF16>(op, a, s) : launch_fast_op<kF16>(op, a, s))
                            : (a.dtype == kBF16 ? launch_any_op<kBF16>(op, a, s) : launch_any_op<kF16>(op, a, s));
-  return e == hipSuccess && a.split > 1 ? launch_join(a, s) : e;
+  return e == hipSuccess && op == kWgrad && a.split > 1 ? launch_join(a, s) : e;
 }
 
 }  // namespace dsml

@@ -278,6 +278,37 @@ def test_wgrad_of_few_tiles_and_many_rows(sizes, K, N, dt, gather):
     assert none is None and torch.equal(again, got)
 
 
+@pytest.mark.parametrize("sizes,K,N", [([5, 0, 90], 1789, 159), ([1, 3], 3001, 33), ([17] * 70, 1025, 7), ([300, 41], 643, 1001),
+                                       ([0, 0], 999, 5)])
+@pytest.mark.parametrize("dt", [BF, FP])
+def test_odd_products_of_few_tiles_and_long_reductions(sizes, K, N, dt):
+    """Reductions in parts: bias, ReLU and mask applied once to their sum, rows of no
+    group cleared in a fresh result and left in a given one, the same bits every time."""
+    g = _gen(K + N)
+    lead, tail, E = 3, 21, len(sizes)
+    S = lead + sum(sizes) + tail
+    off, used = offsets_of(sizes, lead).to(DEV), slice(lead, S - tail)
+    rows = _rows(g, S, 50)
+    for red, cols, backward in ((K, N, False), (N, K, False), (K, N, True)):
+        x = _rand(g, S if backward else 50, red, dt=dt)
+        w = _rand(g, E, red, cols, dt=dt, scale=red ** -0.5) if backward else _rand(g, E, cols, red, dt=dt, scale=red ** -0.5)
+        bias, mask = _rand(g, E, cols), _rand(g, S, cols, dt=dt)
+        if backward:
+            x[:lead], x[S - tail:] = torch.nan, torch.nan
+            call = lambda out=None: X.grouped_dgrad(x, w, off, mask, out=out)
+            ref, mag = dgrad64(x, w, sizes, mask, lead=lead)
+        else:
+            call = lambda out=None: X.grouped_linear(x, w, off, bias, True, rows, out=out)
+            ref, mag = linear64(x, w, sizes, bias, True, rows, lead=lead)
+        fresh = call()
+        close(fresh[used], ref[used], rounded_tol(ref, mag, red, dt)[used])
+        assert (fresh[:lead] == 0).all() and (fresh[S - tail:] == 0).all()
+        buf = torch.full((S, cols + 3), 7.0, dtype=dt, device=DEV)
+        call(buf[:, 1:1 + cols])
+        assert torch.equal(buf[used, 1:1 + cols], fresh[used])
+        assert (buf[:lead] == 7).all() and (buf[S - tail:] == 7).all() and (buf[:, 0] == 7).all() and (buf[:, 1 + cols:] == 7).all()
+
+
 def test_wgrad_in_parts_in_two_graphs():
     """Each captured call has a workspace of its own; replayed on new values between eager calls."""
     g = _gen(21)
