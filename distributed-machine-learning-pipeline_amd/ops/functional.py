@@ -120,6 +120,25 @@ def _check_grads(grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Ten
         raise RuntimeError("gradients must be on one device")
 
 
+def _check_written_once(grads: Sequence[torch.Tensor], out: Sequence[torch.Tensor]) -> None:
+    """What is written must be written once, and not read as another gradient."""
+    spans = []
+    for g, o in zip(grads, out):
+        size = g.numel() * g.element_size()
+        if size:
+            spans.append((o.data_ptr(), size, True))
+            if o.data_ptr() != g.data_ptr():
+                spans.append((g.data_ptr(), size, False))
+    end_w = end_r = 0
+    for lo, size, write in sorted(spans):
+        if lo < end_w or (write and lo < end_r):
+            raise RuntimeError("clipped gradients must not overlap")
+        if write:
+            end_w = max(end_w, lo + size)
+        else:
+            end_r = max(end_r, lo + size)
+
+
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """``sqrt(sum g^2)`` over every element of every gradient (float32, bfloat16
     or float16, one type, contiguous), as a 0-dim float32 tensor on their device:
@@ -135,7 +154,8 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float =
                     out: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
     """Scale the gradients by ``min(1, max_norm / (norm + eps))`` and return their
     norm before that.  In place, or into the tensors of ``out`` (the gradients
-    then stay as they are).  A norm that is not a number makes every gradient so
+    then stay as they are), of which none may lie over another one or over a
+    gradient, its own in full excepted.  A norm that is not a number makes every gradient so
     too; an infinite one makes them 0 (not a number where they are infinite)."""
     grads = list(grads)
     if grads and grads[0].is_cuda:
@@ -144,9 +164,7 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float =
         if not value >= 0:
             raise RuntimeError(f"{name} must not be negative, got {value}")
     _check_grads(grads, out)
-    written = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in (grads if out is None else out) if t.numel())
-    if any(a + n > b for (a, n), (b, _) in zip(written, written[1:])):
-        raise RuntimeError("clipped gradients must not overlap")
+    _check_written_once(grads, grads if out is None else out)
     norm = _norm_ref(grads)
     coef = torch.clamp(max_norm / (norm + eps), max=1.0).float()
     for g, o in zip(grads, grads if out is None else out):

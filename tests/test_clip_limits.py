@@ -1,0 +1,48 @@
+"""Gradient clipping at its limits: calls that have no answer are refused on the
+host as on the GPU, and results at the ends of the types' ranges are right."""
+import pytest
+import torch
+
+from hipdsml.ops import functional as F
+
+# (gradients, outputs) as ranges of one buffer of 64: each writes a range twice, or
+# writes over a gradient that is read as another one
+OVERLAPS = {
+    "twice": ([(0, 32), (0, 32)], None),
+    "partly": ([(0, 40), (32, 64)], None),
+    "out over its own, moved": ([(0, 32)], [(16, 48)]),
+    "outs": ([(0, 16), (16, 32)], [(32, 48), (40, 56)]),
+    "out over the next": ([(0, 16), (16, 32)], [(16, 32), (32, 48)]),
+    "out over the one before": ([(0, 16), (16, 32)], [(32, 48), (0, 16)]),
+    "out over two": ([(0, 16), (16, 32), (32, 48)], [(48, 64), (8, 24), (32, 48)]),
+}
+APART = {
+    "in place": ([(0, 32), (32, 64)], None),
+    "one in place, one not": ([(0, 16), (16, 32)], [(0, 16), (32, 48)]),
+    "all moved": ([(0, 16), (16, 32)], [(48, 64), (32, 48)]),
+    "none in it": ([(0, 16), (8, 8), (16, 32)], [(0, 16), (4, 4), (16, 32)]),
+}
+
+
+def _views(buf, spans):
+    return None if spans is None else [buf[a:b] for a, b in spans]
+
+
+@pytest.mark.parametrize("case", sorted(OVERLAPS))
+def test_host_refuses_outputs_over_gradients(case):
+    grads, out = OVERLAPS[case]
+    buf = torch.arange(64, dtype=torch.float32)
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        F.clip_grad_norm_(_views(buf, grads), 1.0, out=_views(buf, out))
+    assert torch.equal(buf, torch.arange(64, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("case", sorted(APART))
+def test_host_takes_ranges_that_lie_apart(case):
+    grads, out = APART[case]
+    buf = torch.arange(64, dtype=torch.float32)
+    want = [buf[a:b].double() for a, b in grads]
+    n = float(F.clip_grad_norm_(_views(buf, grads), 1.0, out=_views(buf, out)))
+    for (a, b), g in zip(grads if out is None else out, want):
+        # the roundings of the norm, the factor and the product
+        assert ((buf[a:b] - g / (n + 1e-6)).abs() <= g / n * 2.0 ** -22).all()
