@@ -20,6 +20,9 @@ captured into a graph.  The gradients are the explicit calls above (autograd doe
 not record a call's kernels).  Products take bfloat16 or float16 with fp32 sums; weight
 and bias gradients are float32, as the trainers keep them.
 
+A result buffer (``out``, ``dw``, ``db``) may not overlap an operand or another
+result; column ranges of one buffer, and pieces that only touch, lie apart.
+
 GPU tensors go to the HIP kernels (mandatory), host tensors to the same math in
 PyTorch.  A call runs on its tensors' device, on that device's current stream.
 Offsets and rows are not checked on the host (that would wait for the GPU): the
@@ -75,6 +78,33 @@ def _out2(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, name: str =
     _check(t.dtype == like.dtype, f"{name} must have the operands' type")
     _check(tuple(t.shape) == (rows, cols), f"{name} must be [{rows}, {cols}]")
     _check(rows <= 1 or t.stride(0) >= cols, f"{name}: rows must not overlap")
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """The bytes from the first element to behind the last."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _meets(a: torch.Tensor, b: torch.Tensor) -> bool:
+    (alo, ahi), (blo, bhi) = _span(a), _span(b)
+    if alo >= bhi or blo >= ahi:
+        return False
+    # column ranges of one buffer lie apart though their spans do not
+    if a.dim() != 2 or b.dim() != 2:
+        return True
+    ea, eb = a.element_size(), b.element_size()
+    ld = a.stride(0) * ea if a.shape[0] > 1 else b.stride(0) * eb
+    if ld <= 0 or (b.shape[0] > 1 and b.stride(0) * eb != ld):
+        return True
+    at = (blo - alo) % ld  # b's first column, from a's
+    return at < a.shape[1] * ea or at + b.shape[1] * eb > ld
+
+
+def _apart(out: torch.Tensor, *ins: Optional[torch.Tensor], name: str = "out") -> None:
+    _check(all(t is None or not _meets(out, t) for t in ins), f"{name} must not overlap an input")
 
 
 def _host(*ts: Optional[torch.Tensor]) -> None:
@@ -216,6 +246,7 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias
     S = x.shape[0] if rows is None else rows.numel()
     if out is not None:
         _out2(out, S, N, x)
+        _apart(out, x, w, offsets, bias, rows)
     y = torch.zeros(S, N, dtype=x.dtype) if out is None else out
     xs = _take(x, rows)
     for e, a, b in _groups(offsets, S):
@@ -249,6 +280,7 @@ def grouped_dgrad(dz: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, mask
         _check(tuple(mask.shape) == (S, K), f"mask must be [{S}, {K}]")
     if out is not None:
         _out2(out, S, K, dz)
+        _apart(out, dz, w, offsets, mask)
     dx = torch.zeros(S, K, dtype=dz.dtype) if out is None else out
     for e, a, b in _groups(offsets, S):
         z = dz[a:b].float() @ w[e].float()
@@ -285,11 +317,13 @@ def grouped_wgrad(dz: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, rows
         _check(tuple(dw.shape) == (E, N, K), f"dw must be [{E}, {N}, {K}]")
         _check((N <= 1 or dw.stride(1) >= K) and (E <= 1 or dw.stride(0) >= (N - 1) * dw.stride(1) + K),
                "dw: rows must not overlap")
-    else:
-        dw = torch.empty(E, N, K)
+        _apart(dw, dz, x, offsets, rows, db, name="dw")
     if db is not None:
         _f32(db, E * N, "db")
-    elif bias:
+        _apart(db, dz, x, offsets, rows, name="db")
+    if dw is None:
+        dw = torch.empty(E, N, K)
+    if db is None and bias:
         db = torch.empty(E, N)
     xs, d = _take(x, rows), dz.float()
     for e, a, b in _groups(offsets, S):
@@ -315,6 +349,7 @@ def expert_combine(y: torch.Tensor, route: Route, weighted: bool = True,
     _i32(route.slots, T * k, "slots")
     if out is not None:
         _out2(out, T, y.shape[1], y)
+        _apart(out, y, route.slots, gates)
     acc = torch.zeros(T, y.shape[1])
     for j in range(k):
         v, s = _take(y, route.slots[:, j]), route.slots[:, j:j + 1]

@@ -1,0 +1,110 @@
+"""Expert-layer calls that have no right answer are refused on the host as on the
+GPU (the native checks come before any launch, so host tensors reach them)."""
+import pytest
+import torch
+
+from hipdsml.ops import experts as X
+from hipdsml.ops.native import load_native
+
+BF = torch.bfloat16
+OFF = torch.tensor([0, 2, 4], dtype=torch.int32)
+
+
+def _native():
+    C = load_native()
+    if C is None:
+        pytest.skip("extension not built")
+    return C
+
+
+def _call(side, name, **kw):
+    """The public call, or the native one with the same arguments."""
+    if side == "host":
+        return getattr(X, name)(**kw)
+    if name == "expert_combine":
+        r, weighted = kw.pop("route"), kw.pop("weighted", True)
+        kw.update(slots=r.slots, gates=r.gates if weighted else None)
+    if name == "expert_combine_backward":
+        r = kw.pop("route")
+        kw.update(slots=r.slots, gates=r.gates, offsets=r.offsets)
+    return getattr(_native(), name)(**kw)
+
+
+# 4 slots, 2 experts [4 out, 8 in], as pieces of one buffer `b` of 256 elements
+def _x(b):
+    return b[:32].view(4, 8)
+
+
+def _dz(b):
+    return b[:16].view(4, 4)
+
+
+def _w(b):
+    return b[64:128].view(2, 4, 8)
+
+
+def _f32(b, lo, *shape):
+    return b.view(torch.float32)[lo:].as_strided(shape, torch.empty(shape).stride())
+
+
+OVER = {
+    "linear out, x": ("grouped_linear", lambda b: dict(x=_x(b), w=_w(b), offsets=OFF, out=b[16:32].view(4, 4))),
+    "linear out, weights": ("grouped_linear", lambda b: dict(x=_x(b), w=_w(b), offsets=OFF, out=b[100:116].view(4, 4))),
+    "linear out, bias": ("grouped_linear", lambda b: dict(x=_x(b), w=_w(b), offsets=OFF, bias=_f32(b, 64, 2, 4),
+                                                          out=b[140:156].view(4, 4))),
+    "linear out, offsets": ("grouped_linear", lambda b: dict(x=_x(b), w=_w(b), offsets=b.view(torch.int32)[64:67],
+                                                             out=b[128:144].view(4, 4))),
+    "linear out, rows": ("grouped_linear", lambda b: dict(x=_x(b), w=_w(b), offsets=OFF, rows=b.view(torch.int32)[64:68],
+                                                          out=b[134:150].view(4, 4))),
+    "linear columns": ("grouped_linear", lambda b: dict(x=b[128:192].view(4, 16)[:, :8], w=_w(b), offsets=OFF,
+                                                        out=b[128:192].view(4, 16)[:, 7:11])),
+    "dgrad out, dz": ("grouped_dgrad", lambda b: dict(dz=_dz(b), w=_w(b), offsets=OFF, out=b[12:44].view(4, 8))),
+    "dgrad out, weights": ("grouped_dgrad", lambda b: dict(dz=_dz(b), w=_w(b), offsets=OFF, out=b[96:128].view(4, 8))),
+    "dgrad out, mask": ("grouped_dgrad", lambda b: dict(dz=_dz(b), w=_w(b), offsets=OFF, mask=b[128:160].view(4, 8),
+                                                        out=b[128:160].view(4, 8))),
+    "wgrad dw, dz": ("grouped_wgrad", lambda b: dict(dz=_dz(b), x=_w(b)[0], offsets=OFF, dw=_f32(b, 7, 2, 4, 8))),
+    "wgrad dw, x": ("grouped_wgrad", lambda b: dict(dz=_dz(b), x=b[150:182].view(4, 8), offsets=OFF,
+                                                    dw=_f32(b, 16, 2, 4, 8))),
+    "wgrad db, dz": ("grouped_wgrad", lambda b: dict(dz=_dz(b), x=_w(b)[0], offsets=OFF, db=_f32(b, 4, 2, 4))),
+    "wgrad dw, db": ("grouped_wgrad", lambda b: dict(dz=_dz(b), x=b[16:48].view(4, 8), offsets=OFF,
+                                                     dw=_f32(b, 64, 2, 4, 8), db=_f32(b, 120, 2, 4))),
+    "combine out, y": ("expert_combine", lambda b: dict(y=_x(b), route=_route(), out=b[8:24].view(2, 8))),
+    "combine out, gates": ("expert_combine", lambda b: dict(y=_x(b), route=_route(gates=_f32(b, 64, 2, 2)),
+                                                            out=b[130:146].view(2, 8))),
+}
+
+
+def _route(**kw):
+    r = X.Route(torch.full((2, 2), 0.5), torch.tensor([[0, 1], [0, 1]], dtype=torch.int32), OFF,
+                torch.tensor([0, 1, 0, 1], dtype=torch.int32), torch.tensor([[0, 2], [1, 3]], dtype=torch.int32))
+    return r._replace(**kw)
+
+
+@pytest.mark.parametrize("side", ["host", "native"])
+@pytest.mark.parametrize("case", sorted(OVER))
+def test_results_over_operands_are_refused(case, side):
+    name, make = OVER[case]
+    buf = torch.zeros(256, dtype=BF)
+    with pytest.raises(RuntimeError, match="must not overlap an input"):
+        _call(side, name, **make(buf))
+    assert (buf == 0).all()
+
+
+def test_results_beside_operands_are_taken():
+    """Columns of one buffer, and pieces that touch: the same results as apart."""
+    g = torch.Generator().manual_seed(3)
+    buf = torch.randn(4, 24, generator=g).to(BF)
+    w = torch.randn(2, 8, 16, generator=g).to(BF)
+    want = X.grouped_linear(buf[:, :16].clone(), w, OFF)
+    X.grouped_linear(buf[:, :16], w, OFF, out=buf[:, 16:])
+    assert torch.equal(buf[:, 16:], want)
+    flat = torch.zeros(4 * 8 + 4 * 16, dtype=BF)
+    dz, out = flat[:32].view(4, 8), flat[32:].view(4, 16)
+    dz.copy_(want)
+    X.grouped_dgrad(dz, w, OFF, out=out)
+    assert torch.equal(out, X.grouped_dgrad(want, w, OFF)) and torch.equal(dz, want)
+    f = torch.zeros(2 * 8 * 16 + 2 * 8)
+    dw, db = f[:256].view(2, 8, 16), f[256:].view(2, 8)
+    X.grouped_wgrad(dz, out, OFF, dw=dw, db=db)
+    for a, b in zip((dw, db), X.grouped_wgrad(dz, out, OFF)):
+        assert torch.equal(a, b)
