@@ -80,6 +80,26 @@ def _out2(t: torch.Tensor, rows: int, cols: int, like: torch.Tensor, name: str =
     _check(rows <= 1 or t.stride(0) >= cols, f"{name}: rows must not overlap")
 
 
+def _count(n: int, what: str) -> None:
+    _check(n <= 0x7FFFFFFF, f"{what}: more than 2^31 - 1 rows")
+
+
+def _weights(w: torch.Tensor) -> None:
+    _rows2(w, 3, "w")
+    E, N, K = w.shape
+    _check(min(E, N, K) >= 1, "w must be [experts, out, in], none of them 0")
+    _check(max(N, K) <= 0xFFFFFF and E <= 0xFFFF, "w is too large in one axis")
+
+
+def _slots(slots: torch.Tensor, what: str) -> Tuple[int, int]:
+    _check(slots.dim() == 2, f"slots must have 2 axes, got {slots.dim()}")
+    T, k = slots.shape
+    _check(1 <= k <= MAX_K, f"{what}: k must be 1..{MAX_K}, got {k}")
+    _count(T * k, what)
+    _i32(slots, T * k, "slots")
+    return T, k
+
+
 def _span(t: torch.Tensor) -> Tuple[int, int]:
     """The bytes from the first element to behind the last."""
     if t.numel() == 0:
@@ -128,17 +148,18 @@ def route_topk(logits: torch.Tensor, k: int, normalize: str = "topk") -> Route:
     return _route_ref(logits, index(k), normalize)
 
 
-def _check_route(T: int, E: int, k: int, normalize: str) -> None:
+def _check_route(T: int, E: int, k: int, normalize: str, logits: torch.Tensor) -> None:
     _check(1 <= E <= MAX_EXPERTS, f"route_topk: 1..{MAX_EXPERTS} experts, got {E}")
     _check(1 <= k <= min(E, MAX_K), f"route_topk: k must be 1..min({MAX_K}, experts), got {k}")
+    _count(T * k, "route_topk")
     _check(normalize in ("topk", "all"), f"normalize must be 'topk' or 'all', got {normalize!r}")
+    _check(logits.dtype in (torch.float32,) + _HALF, "logits must be float32, bfloat16 or float16")
 
 
 def _route_ref(logits: torch.Tensor, k: int, normalize: str) -> Route:
     _rows2(logits, 2, "logits")
     T, E = logits.shape
-    _check_route(T, E, k, normalize)
-    _check(logits.dtype in (torch.float32,) + _HALF, "logits must be float32, bfloat16 or float16")
+    _check_route(T, E, k, normalize, logits)
     x = logits.float()
     x = torch.where(x.isnan(), torch.full_like(x, -torch.inf), x)
     val, ids = torch.sort(x, dim=1, descending=True, stable=True)
@@ -174,7 +195,7 @@ def route_topk_backward(dgates: torch.Tensor, logits: torch.Tensor, route: Route
     T, E = logits.shape
     _check(dgates.dim() == 2, f"dgates must have 2 axes, got {dgates.dim()}")
     k = dgates.shape[1]
-    _check_route(T, E, k, normalize)
+    _check_route(T, E, k, normalize, logits)
     for t, name in ((dgates, "dgates"), (route.gates, "gates")):
         _f32(t, T * k, name)
     _i32(route.experts, T * k, "experts")
@@ -229,9 +250,8 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias
         return require_native().grouped_linear(x, w, offsets, bias, relu, rows, out)
     _host(w, offsets, bias, rows, out)
     _rows2(x, 2, "x")
-    _rows2(w, 3, "w")
+    _weights(w)
     E, N, K = w.shape
-    _check(min(E, N, K) >= 1, "w must be [experts, out, in], none of them 0")
     _check(x.dtype in _HALF, "x must be bfloat16 or float16")
     _check(w.dtype == x.dtype, "w must have x's type")
     _check(x.shape[1] == K, f"x has {x.shape[1]} columns, w takes {K}")
@@ -244,6 +264,7 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias
         _check(bias.dtype == torch.float32, "bias must be float32")
         _check(tuple(bias.shape) == (E, N), f"bias must be [{E}, {N}]")
     S = x.shape[0] if rows is None else rows.numel()
+    _count(max(S, x.shape[0]), "grouped_linear")
     if out is not None:
         _out2(out, S, N, x)
         _apart(out, x, w, offsets, bias, rows)
@@ -266,14 +287,14 @@ def grouped_dgrad(dz: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, mask
         return require_native().grouped_dgrad(dz, w, offsets, mask, out)
     _host(w, offsets, mask, out)
     _rows2(dz, 2, "dz")
-    _rows2(w, 3, "w")
+    _weights(w)
     E, N, K = w.shape
-    _check(min(E, N, K) >= 1, "w must be [experts, out, in], none of them 0")
     _check(dz.dtype in _HALF, "dz must be bfloat16 or float16")
     _check(w.dtype == dz.dtype, "w must have dz's type")
     _check(dz.shape[1] == N, f"dz has {dz.shape[1]} columns, w gives {N}")
     _i32(offsets, E + 1, "offsets")
     S = dz.shape[0]
+    _count(S, "grouped_dgrad")
     if mask is not None:
         _rows2(mask, 2, "mask")
         _check(mask.dtype == dz.dtype, "mask must have dz's type")
@@ -305,11 +326,13 @@ def grouped_wgrad(dz: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, rows
     _check(offsets.dim() == 1 and offsets.numel() >= 2, "offsets must have 1 axis and hold experts + 1 values")
     E, (S, N), K = offsets.numel() - 1, dz.shape, x.shape[1]
     _i32(offsets, E + 1, "offsets")
+    _check(min(N, K) >= 1 and max(N, K) <= 0xFFFFFF and E <= 0xFFFF, "grouped_wgrad: bad sizes")
     if rows is not None:
         _check(rows.dim() == 1, "rows must have 1 axis")
         _i32(rows, S, "rows")
     else:
         _check(x.shape[0] == S, f"x has {x.shape[0]} rows, dz {S}")
+    _count(max(S, x.shape[0]), "grouped_wgrad")
     _check(bias or db is None, "a bias gradient buffer was given with bias=False")
     if dw is not None:
         _rows2(dw, 3, "dw")
@@ -345,8 +368,11 @@ def expert_combine(y: torch.Tensor, route: Route, weighted: bool = True,
     _host(*route, out)
     _rows2(y, 2, "y")
     _check(y.dtype in _HALF, "y must be bfloat16 or float16")
-    T, k = route.slots.shape
-    _i32(route.slots, T * k, "slots")
+    T, k = _slots(route.slots, "expert_combine")
+    _check(1 <= y.shape[1] <= 0x3FFFFF, "expert_combine: 1..4194303 columns")
+    _count(y.shape[0], "expert_combine")
+    if weighted:
+        _f32(gates, T * k, "gates")
     if out is not None:
         _out2(out, T, y.shape[1], y)
         _apart(out, y, route.slots, gates)
@@ -373,10 +399,13 @@ def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor,
     _rows2(y, 2, "y")
     _check(y.dtype in _HALF, "y must be bfloat16 or float16")
     _check(dout.dtype == y.dtype, "dout must have y's type")
-    T, k = route.slots.shape
+    T, k = _slots(route.slots, "expert_combine_backward")
     S, N = y.shape
-    _i32(route.slots, T * k, "slots")
+    _check(1 <= N <= 0x3FFFFF, "expert_combine_backward: 1..4194303 columns")
     _f32(route.gates, T * k, "gates")
+    _check(route.offsets.dim() == 1 and route.offsets.numel() >= 2,
+           "offsets must have 1 axis and hold experts + 1 values")
+    _i32(route.offsets, route.offsets.numel(), "offsets")
     _check(tuple(dout.shape) == (T, N), f"dout must be [{T}, {N}]")
     _check(S == T * k, f"y must have one row a slot: {T * k}, got {S}")
     d = dout.float()

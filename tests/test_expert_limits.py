@@ -108,3 +108,58 @@ def test_results_beside_operands_are_taken():
     X.grouped_wgrad(dz, out, OFF, dw=dw, db=db)
     for a, b in zip((dw, db), X.grouped_wgrad(dz, out, OFF)):
         assert torch.equal(a, b)
+
+
+BAD_ARGUMENTS = {
+    "combine gates type": ("expert_combine", lambda: dict(y=torch.ones(4, 8, dtype=BF), route=_route(
+        gates=torch.ones(2, 2, dtype=torch.float64))), "gates must be float32"),
+    "combine gates size": ("expert_combine", lambda: dict(y=torch.ones(4, 8, dtype=BF), route=_route(
+        gates=torch.ones(3, 2))), "gates must hold 4"),
+    "combine gates strided": ("expert_combine", lambda: dict(y=torch.ones(4, 8, dtype=BF), route=_route(
+        gates=torch.ones(2, 2).t())), "gates must be contiguous"),
+    "combine slots axes": ("expert_combine", lambda: dict(y=torch.ones(4, 8, dtype=BF), weighted=False, route=_route(
+        slots=torch.zeros(4, dtype=torch.int32))), "slots must have 2 axes"),
+    "combine choices": ("expert_combine", lambda: dict(y=torch.ones(4, 8, dtype=BF), weighted=False, route=_route(
+        slots=torch.zeros(2, 17, dtype=torch.int32))), "k must be 1..16"),
+    "combine no choices": ("expert_combine", lambda: dict(y=torch.ones(4, 8, dtype=BF), weighted=False, route=_route(
+        slots=torch.zeros(2, 0, dtype=torch.int32))), "k must be 1..16"),
+    "combine columns": ("expert_combine", lambda: dict(y=torch.ones(4, 0, dtype=BF), route=_route()), "columns"),
+    "backward choices": ("expert_combine_backward", lambda: dict(
+        dout=torch.ones(2, 8, dtype=BF), y=torch.ones(34, 8, dtype=BF),
+        route=_route(slots=torch.zeros(2, 17, dtype=torch.int32), gates=torch.ones(2, 17))), "k must be 1..16"),
+    "backward columns": ("expert_combine_backward", lambda: dict(
+        dout=torch.ones(2, 0, dtype=BF), y=torch.ones(4, 0, dtype=BF), route=_route()), "columns"),
+    "backward offsets": ("expert_combine_backward", lambda: dict(
+        dout=torch.ones(2, 8, dtype=BF), y=torch.ones(4, 8, dtype=BF), route=_route(offsets=OFF[:1])), "experts \\+ 1"),
+    "backward offsets type": ("expert_combine_backward", lambda: dict(
+        dout=torch.ones(2, 8, dtype=BF), y=torch.ones(4, 8, dtype=BF), route=_route(offsets=OFF.long())), "int32"),
+    "wgrad columns": ("grouped_wgrad", lambda: dict(dz=torch.ones(4, 0, dtype=BF), x=torch.ones(4, 8, dtype=BF),
+                                                    offsets=OFF), "bad sizes"),
+    "wgrad width": ("grouped_wgrad", lambda: dict(dz=torch.ones(4, 4, dtype=BF), x=torch.ones(4, 0, dtype=BF),
+                                                  offsets=OFF), "bad sizes"),
+    "linear size": ("grouped_linear", lambda: dict(
+        x=torch.ones(1, 1, dtype=BF), w=torch.ones(1, 1, 1, dtype=BF).expand(1, 1 << 24, 1), offsets=OFF[:2]), "too large"),
+    "linear rows": ("grouped_linear", lambda: dict(
+        x=torch.ones(1, 8, dtype=BF).expand(1 << 31, 8), w=torch.ones(2, 4, 8, dtype=BF), offsets=OFF), "more than 2\\^31"),
+    "dgrad rows": ("grouped_dgrad", lambda: dict(
+        dz=torch.ones(1, 4, dtype=BF).expand(1 << 31, 4), w=torch.ones(2, 4, 8, dtype=BF), offsets=OFF), "more than 2\\^31"),
+}
+
+
+@pytest.mark.parametrize("side", ["host", "native"])
+@pytest.mark.parametrize("case", sorted(BAD_ARGUMENTS))
+def test_arguments_are_refused_alike(case, side):
+    name, make, msg = BAD_ARGUMENTS[case]
+    with pytest.raises(RuntimeError, match=msg):
+        _call(side, name, **make())
+
+
+@pytest.mark.parametrize("side", ["host", "native"])
+def test_route_backward_takes_the_routers_types(side):
+    logits = torch.randn(3, 8)
+    r = X.route_topk(logits, 2)
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        if side == "host":
+            X.route_topk_backward(torch.zeros(3, 2), logits.double(), r)
+        else:
+            _native().route_topk_backward(torch.zeros(3, 2), logits.double(), r.gates, r.experts)
