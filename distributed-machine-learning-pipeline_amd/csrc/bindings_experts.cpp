@@ -51,6 +51,16 @@ void check_gpu(std::initializer_list<const torch::Tensor*> ts) {
   }
 }
 
+// No call here is recorded by autograd: an operand that requires a gradient would
+// lose it without a word.
+void check_unrecorded(std::initializer_list<const torch::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const torch::Tensor* t : ts)
+    TORCH_CHECK(!t || !t->requires_grad(),
+                "an operand requires a gradient, and autograd does not record this call: make it under "
+                "torch.no_grad(), with the explicit gradient calls, or detach the operand");
+}
+
 int32_t half_type(const torch::Tensor& t, const char* name) {
   if (t.scalar_type() == torch::kBFloat16) return kBF16;
   TORCH_CHECK(t.scalar_type() == torch::kFloat16, name, " must be bfloat16 or float16");
@@ -119,6 +129,7 @@ bool whole_row(const std::string& normalize) {
 
 // ---- router -------------------------------------------------------------
 py::tuple py_route_topk(const torch::Tensor& logits, int64_t k, const std::string& normalize) {
+  check_unrecorded({&logits});
   check_rows(logits, 2, "logits");
   const int64_t T = logits.size(0), E = logits.size(1);
   TORCH_CHECK(E >= 1 && E <= kRouteMaxExperts, "route_topk: 1..", kRouteMaxExperts, " experts, got ", E);
@@ -147,6 +158,7 @@ py::tuple py_route_topk(const torch::Tensor& logits, int64_t k, const std::strin
 
 torch::Tensor py_route_backward(const torch::Tensor& dgates, const torch::Tensor& logits, const torch::Tensor& gates,
                                 const torch::Tensor& experts, const std::string& normalize) {
+  check_unrecorded({&logits, &dgates, &gates});
   check_rows(logits, 2, "logits");
   TORCH_CHECK(dgates.dim() == 2, "dgates must have 2 axes, got ", dgates.dim());
   const int64_t T = logits.size(0), E = logits.size(1), k = dgates.size(1);
@@ -189,6 +201,7 @@ void run_grouped(GroupedOp op, GroupedArgs& a, const torch::Tensor& like, const 
 
 torch::Tensor py_grouped_linear(const torch::Tensor& x, const torch::Tensor& w, const torch::Tensor& offsets,
                                 const Opt& bias, bool relu, const Opt& rows, const Opt& out) {
+  check_unrecorded({&x, &w, opt(bias), opt(out)});
   check_rows(x, 2, "x");
   check_weights(w);
   const int64_t E = w.size(0), N = w.size(1), K = w.size(2);
@@ -229,6 +242,7 @@ torch::Tensor py_grouped_linear(const torch::Tensor& x, const torch::Tensor& w, 
 
 torch::Tensor py_grouped_dgrad(const torch::Tensor& dz, const torch::Tensor& w, const torch::Tensor& offsets,
                                const Opt& mask, const Opt& out) {
+  check_unrecorded({&dz, &w, opt(mask), opt(out)});
   check_rows(dz, 2, "dz");
   check_weights(w);
   const int64_t E = w.size(0), N = w.size(1), K = w.size(2), S = dz.size(0);
@@ -262,6 +276,7 @@ torch::Tensor py_grouped_dgrad(const torch::Tensor& dz, const torch::Tensor& w, 
 
 py::tuple py_grouped_wgrad(const torch::Tensor& dz, const torch::Tensor& x, const torch::Tensor& offsets,
                            const Opt& rows, bool bias, const Opt& dw_out, const Opt& db_out) {
+  check_unrecorded({&dz, &x, opt(dw_out), opt(db_out)});
   check_rows(dz, 2, "dz");
   check_rows(x, 2, "x");
   GroupedArgs a{};
@@ -319,6 +334,7 @@ void check_slots(const torch::Tensor& slots, int64_t* T, int64_t* k, const char*
 }
 
 torch::Tensor py_combine(const torch::Tensor& y, const torch::Tensor& slots, const Opt& gates, const Opt& out) {
+  check_unrecorded({&y, opt(gates), opt(out)});
   check_rows(y, 2, "y");
   CombineArgs a{};
   a.dtype = half_type(y, "y");
@@ -346,6 +362,7 @@ torch::Tensor py_combine(const torch::Tensor& y, const torch::Tensor& slots, con
 
 py::tuple py_combine_backward(const torch::Tensor& dout, const torch::Tensor& y, const torch::Tensor& slots,
                               const torch::Tensor& gates, const torch::Tensor& offsets) {
+  check_unrecorded({&dout, &y, &gates});
   check_rows(dout, 2, "dout");
   check_rows(y, 2, "y");
   CombineBwdArgs a{};
@@ -383,6 +400,7 @@ torch::Tensor py_grad_norm(const std::vector<torch::Tensor>& grads, bool clip, d
   bool gpu = true;
   for (size_t i = 0; i < grads.size(); ++i) {
     const torch::Tensor& g = grads[i];
+    check_unrecorded({&g, out ? &(*out)[i] : nullptr});
     TORCH_CHECK(g.scalar_type() == grads[0].scalar_type(), "gradients must have one type");
     TORCH_CHECK(g.is_contiguous(), "gradients must be contiguous");
     const torch::Tensor& o = out ? (*out)[i] : g;

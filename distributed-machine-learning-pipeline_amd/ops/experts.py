@@ -16,8 +16,9 @@ experts, each token going through the k experts its router chose.
 A token's choice owns a *slot*; slots are ordered by expert, then by token, and
 expert e owns the slots ``offsets[e] .. offsets[e + 1] - 1``.  The plan lives on
 the GPU: nothing here synchronises or copies to the host, and every call can be
-captured into a graph.  The gradients are the explicit calls above (autograd does
-not record a call's kernels).  Products take bfloat16 or float16 with fp32 sums; weight
+captured into a graph.  The gradients are the explicit calls above: autograd does
+not record a call, so where gradients are recorded an operand that requires one is
+refused (parameters are taken under ``torch.no_grad()``).  Products take bfloat16 or float16 with fp32 sums; weight
 and bias gradients are float32, as the trainers keep them.
 
 A result buffer (``out``, ``dw``, ``db``) may not overlap an operand or another
@@ -36,6 +37,7 @@ from typing import NamedTuple, Optional, Tuple
 
 import torch
 
+from .functional import check_unrecorded
 from .native import require_native
 
 MAX_EXPERTS, MAX_K = 512, 16
@@ -145,6 +147,7 @@ def route_topk(logits: torch.Tensor, k: int, normalize: str = "topk") -> Route:
     """
     if logits.is_cuda:
         return Route(*require_native().route_topk(logits, index(k), normalize))
+    check_unrecorded(logits)
     return _route_ref(logits, index(k), normalize)
 
 
@@ -190,6 +193,7 @@ def route_topk_backward(dgates: torch.Tensor, logits: torch.Tensor, route: Route
     the whole row's softmax for ``"all"``."""
     if logits.is_cuda:
         return require_native().route_topk_backward(dgates, logits, route.gates, route.experts, normalize)
+    check_unrecorded(dgates, logits, route.gates)
     _host(dgates, *route)
     _rows2(logits, 2, "logits")
     T, E = logits.shape
@@ -248,6 +252,7 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, bias
     """
     if x.is_cuda:
         return require_native().grouped_linear(x, w, offsets, bias, relu, rows, out)
+    check_unrecorded(x, w, bias, out)
     _host(w, offsets, bias, rows, out)
     _rows2(x, 2, "x")
     _weights(w)
@@ -285,6 +290,7 @@ def grouped_dgrad(dz: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, mask
     ``expert_combine(dx, route, weighted=False)`` sums a token's slots."""
     if dz.is_cuda:
         return require_native().grouped_dgrad(dz, w, offsets, mask, out)
+    check_unrecorded(dz, w, mask, out)
     _host(w, offsets, mask, out)
     _rows2(dz, 2, "dz")
     _weights(w)
@@ -318,6 +324,7 @@ def grouped_wgrad(dz: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, rows
     leaves the bias gradient out (None)."""
     if dz.is_cuda:
         return require_native().grouped_wgrad(dz, x, offsets, rows, bias, dw, db)
+    check_unrecorded(dz, x, dw, db)
     _host(x, offsets, rows, dw, db)
     _rows2(dz, 2, "dz")
     _rows2(x, 2, "x")
@@ -365,6 +372,7 @@ def expert_combine(y: torch.Tensor, route: Route, weighted: bool = True,
     gates = route.gates if weighted else None
     if y.is_cuda:
         return require_native().expert_combine(y, route.slots, gates, out)
+    check_unrecorded(y, gates, out)
     _host(*route, out)
     _rows2(y, 2, "y")
     _check(y.dtype in _HALF, "y must be bfloat16 or float16")
@@ -394,6 +402,7 @@ def expert_combine_backward(dout: torch.Tensor, y: torch.Tensor,
     <dout[t], y[slot]>`` in float32.  A slot belongs to one choice."""
     if y.is_cuda:
         return require_native().expert_combine_backward(dout, y, route.slots, route.gates, route.offsets)
+    check_unrecorded(dout, y, route.gates)
     _host(dout, *route)
     _rows2(dout, 2, "dout")
     _rows2(y, 2, "y")

@@ -96,11 +96,20 @@ def scale_(x: torch.Tensor, alpha: float) -> torch.Tensor:
     return x
 
 
+def check_unrecorded(*ts: Optional[torch.Tensor]) -> None:
+    """Refuse operands that require a gradient where gradients are recorded: the
+    kernels are not, and the gradient would be lost without a word."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError("an operand requires a gradient, and autograd does not record this call: make it under "
+                           "torch.no_grad(), with the explicit gradient calls, or detach the operand")
+
+
 def _norm_ref(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     return sum(g.double().square().sum() for g in grads).sqrt()
 
 
 def _check_grads(grads: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]]) -> None:
+    check_unrecorded(*grads, *(out or []))
     if not grads:
         raise RuntimeError("no gradients given")
     if grads[0].dtype not in (torch.float32, torch.bfloat16, torch.float16):
@@ -142,7 +151,9 @@ def _check_written_once(grads: Sequence[torch.Tensor], out: Sequence[torch.Tenso
 def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
     """``sqrt(sum g^2)`` over every element of every gradient (float32, bfloat16
     or float16, one type, contiguous), as a 0-dim float32 tensor on their device:
-    nothing is copied to the host.  Squares are summed in float64."""
+    nothing is copied to the host.  Squares are summed in float64.  Autograd does
+    not record it: tensors that require a gradient are refused where gradients are
+    recorded."""
     grads = list(grads)
     if grads and grads[0].is_cuda:
         return require_native().grad_norm(grads)
@@ -152,11 +163,12 @@ def grad_norm(grads: Sequence[torch.Tensor]) -> torch.Tensor:
 
 def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float = 1e-6,
                     out: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
-    """Scale the gradients by ``min(1, max_norm / (norm + eps))`` and return their
-    norm before that.  In place, or into the tensors of ``out`` (the gradients
-    then stay as they are), of which none may lie over another one or over a
-    gradient, its own in full excepted.  A norm that is not a number makes every gradient so
-    too; an infinite one makes them 0 (not a number where they are infinite)."""
+    """Scale the gradients (tensors as ``grad_norm`` takes them, not the parameters)
+    by ``min(1, max_norm / (norm + eps))`` and return their norm before that.  In
+    place, or into the tensors of ``out`` (the gradients then stay as they are), of
+    which none may lie over another one or over a gradient, its own in full
+    excepted.  A norm that is not a number makes every gradient so too; an infinite
+    one makes them 0 (not a number where they are infinite)."""
     grads = list(grads)
     if grads and grads[0].is_cuda:
         return require_native().grad_norm(grads, True, float(max_norm), float(eps), out)
