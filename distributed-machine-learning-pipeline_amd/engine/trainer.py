@@ -873,11 +873,17 @@ class MlpTrainer:
         return G
 
     def apply_gradients(self, g: torch.Tensor, scale: float = 1.0) -> None:
-        """P -= lr * scale * g (the ApplyGradients RPC; HIP kernel on GPU)."""
-        from ..ops.functional import sgd_update_
+        """P -= lr * scale * g (the ApplyGradients RPC; HIP kernel on GPU).  With
+        clip_norm the norm of scale * g is limited to it; g itself stays."""
+        from ..ops.functional import clip_grad_norm_, sgd_update_
 
         self.synchronize()
-        sgd_update_(self.P, g.to(self.P.device).contiguous(), self.lr * scale)
+        g = g.detach().to(self.P.device).contiguous()
+        if self.clip_norm and scale:
+            by, given = abs(scale), g
+            g = torch.empty_like(given)
+            clip_grad_norm_([given], self.clip_norm / by, eps=1e-6 / by, out=[g])
+        sgd_update_(self.P, g, self.lr * scale)
         self._params_rewritten()
         if self.device.type == "cuda":
             torch.cuda.synchronize(self.device)
