@@ -220,6 +220,9 @@ class MlpTrainer:
                                   stream=self._stream.cuda_stream if self._stream is not None else 0,
                                   follow_torch=self._stream is None)
         self.runner.set_world_size(self.ctx.world_size)
+        if self.clip_norm and self.graph_steps > 0:
+            log.warning("graph_steps=%d is not used with clip_norm: a clipped step is launched eagerly",
+                        self.graph_steps)
         # chunk of the in-house ring all-reduce; <= 0: tuned at init (N > 1)
         self._ring_chunk = int(ring_chunk_bytes)
         self.ring_chunk_sweep_us: Optional[Dict[str, float]] = None
@@ -690,7 +693,9 @@ class MlpTrainer:
             self.runner.set_persist_carry(False)
 
     def _graphs_on(self) -> bool:
-        """Whether train_steps replays hipGraphs for the active sync mode."""
+        """Whether train_steps replays hipGraphs for the active sync mode.  A clipped
+        step is not replayed: the runner's graphs hold its own launches only, and the
+        norm and the scaling come between them from here (_hip_step_clipped)."""
         if self.graph_steps <= 0 or self.runner is None or self.persistent or self.clip_norm:
             return False
         if not self.ctx.is_distributed:

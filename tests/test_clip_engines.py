@@ -40,3 +40,13 @@ def test_without_a_limit_gradients_are_applied_as_they_are():
     want = tr.P - 0.5 * 0.25 * g
     tr.apply_gradients(g, 0.25)
     assert torch.allclose(tr.P, want, rtol=0, atol=2.0 ** -22)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clip,graph_steps,said", [(0.5, 4, True), (0.5, 0, False), (0.0, 4, False)])
+def test_a_clipped_engine_says_that_it_replays_no_graph(clip, graph_steps, said, caplog):
+    with caplog.at_level("WARNING", logger="hipdsml.trainer"):
+        tr = MlpTrainer(SPEC, synthetic_mnist(64, seed=1), batch=16, lr=0.5, seed=3, clip_norm=clip,
+                        graph_steps=graph_steps, ctx=_ctx("cuda"))
+    assert tr._graphs_on() is (graph_steps > 0 and not clip and not tr.persistent)
+    assert any("graph_steps" in r.getMessage() for r in caplog.records) is said
