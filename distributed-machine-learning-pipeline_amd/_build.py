@@ -4,7 +4,8 @@ No hipify, no JIT cache: every ``.hip`` kernel TU and every runtime ``.cpp`` is
 compiled by ``hipcc --offload-arch=gfx950`` into ``<repo>/build/obj`` and
 linked with the PyTorch binding TU into ``<package>/_C.so``, which travels to
 the GPU box with the repository snapshot.  Objects are rebuilt when their
-source or any header under ``csrc/`` is newer.
+source or any header under ``csrc/`` is newer, or when the command that made them
+(recorded beside each) is not today's.
 
 Usage:  python -m hipdsml._build [--force] [-j N] [--measure]
 
@@ -63,11 +64,29 @@ def _headers_mtime() -> float:
     return max((h.stat().st_mtime for h in hs), default=0.0)
 
 
+def _command(src: Path, obj: Path, flags: list[str]) -> list[str]:
+    return [HIPCC] + flags + ["-c", str(src), "-o", str(obj)]
+
+
+def _record(obj: Path) -> Path:
+    """Where the command that made an object is kept."""
+    return obj.with_name(obj.name + ".cmd")
+
+
+def _stale(src: Path, obj: Path, flags: list[str], hdr_t: float) -> bool:
+    if not obj.exists() or obj.stat().st_mtime < max(src.stat().st_mtime, hdr_t):
+        return True
+    rec = _record(obj)
+    return not rec.exists() or rec.read_text() != " ".join(_command(src, obj, flags))
+
+
 def _compile(src: Path, obj: Path, flags: list[str]) -> tuple[Path, str]:
-    cmd = [HIPCC] + flags + ["-c", str(src), "-o", str(obj)]
+    cmd = _command(src, obj, flags)
+    _record(obj).unlink(missing_ok=True)
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
         raise RuntimeError(f"compile failed: {' '.join(cmd)}\n{p.stdout}\n{p.stderr}")
+    _record(obj).write_text(" ".join(cmd))
     return obj, p.stderr
 
 
@@ -109,8 +128,7 @@ def build(force: bool = False, jobs: int | None = None, verbose: bool = False,
         objs.append(obj)
         jobs_todo.append((src, obj, torch_flags))
 
-    stale = [(s, o, f) for (s, o, f) in jobs_todo
-             if force or not o.exists() or o.stat().st_mtime < max(s.stat().st_mtime, hdr_t)]
+    stale = [(s, o, f) for (s, o, f) in jobs_todo if force or _stale(s, o, f, hdr_t)]
     if stale:
         n = jobs or min(len(stale), int(os.environ.get("MAX_JOBS", "8")), os.cpu_count() or 4)
         with ThreadPoolExecutor(max_workers=max(1, n)) as ex:
