@@ -323,6 +323,22 @@ py::tuple py_grouped_wgrad(const torch::Tensor& dz, const torch::Tensor& x, cons
   return py::make_tuple(dw, db);
 }
 
+// Which kernels contiguous, aligned operands of these sizes go to.
+bool py_grouped_whole_words(const std::string& op, int64_t S, int64_t T, int E, int N, int K, bool gathered) {
+  TORCH_CHECK(op == "linear" || op == "dgrad" || op == "wgrad", "op must be 'linear', 'dgrad' or 'wgrad', got '", op, "'");
+  const GroupedOp o = op == "linear" ? kLinear : op == "dgrad" ? kDgrad : kWgrad;
+  const int32_t id = 0;
+  GroupedArgs a{};
+  a.lda = o == kLinear ? K : N;
+  a.ldb = K;
+  a.strb = (int64_t)N * K;
+  a.rows = gathered ? &id : nullptr;
+  a.ldo = o == kLinear ? N : K;
+  a.stro = (int64_t)N * K;
+  a.S = S; a.T = T; a.E = E; a.N = N; a.K = K; a.dtype = kBF16;
+  return grouped_whole_words(o, a);
+}
+
 // ---- combine ---------------------------------------------------------------
 void check_slots(const torch::Tensor& slots, int64_t* T, int64_t* k, const char* what) {
   TORCH_CHECK(slots.dim() == 2, "slots must have 2 axes, got ", slots.dim());
@@ -459,6 +475,9 @@ void bind_experts(py::module_& m) {
         py::arg("mask") = py::none(), py::arg("out") = py::none());
   m.def("grouped_wgrad", &py_grouped_wgrad, py::arg("dz"), py::arg("x"), py::arg("offsets"),
         py::arg("rows") = py::none(), py::arg("bias") = true, py::arg("dw") = py::none(), py::arg("db") = py::none());
+  m.def("grouped_whole_words", &py_grouped_whole_words, py::arg("op"), py::arg("S"), py::arg("T"), py::arg("E"),
+        py::arg("N"), py::arg("K"), py::arg("gathered") = false,
+        "whether contiguous operands of these sizes go to the kernels for whole 16-B words");
   m.def("expert_combine", &py_combine, py::arg("y"), py::arg("slots"), py::arg("gates") = py::none(),
         py::arg("out") = py::none());
   m.def("expert_combine_backward", &py_combine_backward, py::arg("dout"), py::arg("y"), py::arg("slots"),

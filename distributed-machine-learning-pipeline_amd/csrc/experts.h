@@ -70,6 +70,8 @@ struct GroupedArgs {
 };
 enum GroupedOp : int { kLinear = 0, kDgrad = 1, kWgrad = 2 };
 int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a);  // 0: none
+// The kernels for whole 16-B words take the call (else the one for any width).
+bool grouped_whole_words(GroupedOp op, const GroupedArgs& a);
 hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& a, hipStream_t s);
 
 // ---- gated sum of a token's expert rows -------------------------------------

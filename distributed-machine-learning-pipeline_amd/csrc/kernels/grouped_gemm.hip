@@ -201,6 +201,7 @@ typedef uint32_t gg_u4 __attribute__((ext_vector_type(4)));
 // into the last 16 bytes).
 constexpr uint32_t kGgOob = 0xfffffff0u;
 constexpr int64_t kGgSpan = 0xffffff00LL;   // bytes a buffer descriptor may span
+constexpr int64_t kGgIds = 1LL << 29;       // ids a scalar stream can't hold any more
 
 __device__ __forceinline__ gg_u4 gg_desc(const char* base, int64_t bytes) {
   const int64_t b = reinterpret_cast<int64_t>(base);
@@ -1495,6 +1496,8 @@ bool fast_ok(GroupedOp op, const GroupedArgs& a) {
   if (op != kWgrad && a.E > 1 && a.strb % 8) return false;
   if (a.lda > 0x7fffff || a.ldb > 0x7fffff) return false;
   if (op == kLinear && a.rows && (a.T * a.lda + a.K) * 2 > kGgSpan) return false;
+  // a group's ids: 4 bytes each behind offsets and a length of 32 bits
+  if (op == kWgrad && a.rows && a.S >= kGgIds) return false;
   if (op == kWgrad)
     return (!a.rows || (a.T * a.ldb + a.K) * 2 <= kGgSpan) && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 &&
            a.ldo % 4 == 0 && a.ldo <= 0x3fffff && (a.E <= 1 || a.stro % 4 == 0);
@@ -1619,6 +1622,8 @@ int parts_of(GroupedOp op, const GroupedArgs& a) {
   }
   return best;
 }
+
+bool grouped_whole_words(GroupedOp op, const GroupedArgs& a) { return fast_ok(op, a); }
 
 int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a) {
   const int parts = parts_of(op, a);

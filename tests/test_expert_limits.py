@@ -163,3 +163,20 @@ def test_route_backward_takes_the_routers_types(side):
             X.route_topk_backward(torch.zeros(3, 2), logits.double(), r)
         else:
             _native().route_topk_backward(torch.zeros(3, 2), logits.double(), r.gates, r.experts)
+
+
+@pytest.mark.parametrize("S,gathered,whole", [((1 << 29) - 1, True, True), (1 << 29, True, False),
+                                              ((1 << 31) - 256, True, False), (1 << 29, False, True),
+                                              ((1 << 31) - 256, False, True)])
+def test_ids_of_a_weight_gradient_stay_within_32_bits(S, gathered, whole):
+    """The kernel for whole 16-B words streams a group's 4-B ids behind 32-bit offsets, so
+    2^29 of them or more go to the kernel for any width, which indexes in 64."""
+    C = _native()
+    assert C.grouped_whole_words("wgrad", S, 1 << 20, 300, 8, 8, gathered) is whole
+    for op in ("linear", "dgrad"):  # they read an id a lane, in 64 bits
+        assert C.grouped_whole_words(op, S, 1 << 20, 300, 8, 8, op == "linear" and gathered)
+    assert not C.grouped_whole_words("wgrad", 64, 1 << 20, 2, 8, 12, gathered)
+    # a gathered operand is read behind 32-bit offsets too
+    for op in ("linear", "wgrad"):
+        assert C.grouped_whole_words(op, 64, (1 << 28) - 32, 2, 8, 8, True)
+        assert not C.grouped_whole_words(op, 64, 1 << 28, 2, 8, 8, True)
