@@ -292,7 +292,8 @@ py::tuple py_grouped_wgrad(const torch::Tensor& dz, const torch::Tensor& x, cons
   } else {
     TORCH_CHECK(x.size(0) == S, "x has ", x.size(0), " rows, dz ", S);
   }
-  check_count(S, "grouped_wgrad");
+  // the reduction's steps of 64, two ahead of the last, are counted in 32 bits
+  TORCH_CHECK(S <= 0x7fffffffLL - 255, "grouped_wgrad: more than 2^31 - 256 rows");
   check_count(x.size(0), "grouped_wgrad");
   TORCH_CHECK(bias || !db_out, "a bias gradient buffer was given with bias=False");
   if (dw_out) {

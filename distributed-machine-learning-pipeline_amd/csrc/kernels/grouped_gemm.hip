@@ -1634,8 +1634,8 @@ int64_t grouped_ws_floats(GroupedOp op, const GroupedArgs& a) {
 
 hipError_t grouped_gemm(GroupedOp op, const GroupedArgs& args, hipStream_t s) {
   GroupedArgs a = args;
-  if (a.E < 1 || a.N < 1 || a.K < 1 || a.S < 0 || a.T < 0 || a.S > 0x7fffffffLL || a.T > 0x7fffffffLL ||
-      (a.dtype != kBF16 && a.dtype != kF16))
+  if (a.E < 1 || a.N < 1 || a.K < 1 || a.S < 0 || a.T < 0 || a.S > 0x7fffffffLL - (op == kWgrad ? 255 : 0) ||
+      a.T > 0x7fffffffLL || (a.dtype != kBF16 && a.dtype != kF16))
     return hipErrorInvalidValue;
   if (op != kWgrad && a.S == 0) return hipSuccess;
   a.split = parts_of(op, a);

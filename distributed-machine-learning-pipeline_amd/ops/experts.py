@@ -319,7 +319,8 @@ def grouped_wgrad(dz: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, rows
                   bias: bool = True, dw: Optional[torch.Tensor] = None,
                   db: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """``dw[e] = dz_e.T @ x_e`` [E, N, K] and ``db[e]`` = column sums of dz_e
-    [E, N], float32, over the slots of group e (an empty group: zeros).  ``dw``
+    [E, N], float32, over the slots of group e (an empty group: zeros), of which
+    there may be 2^31 - 256 in all.  ``dw``
     / ``db``: buffers to write (dw's rows may be strided); ``bias=False``
     leaves the bias gradient out (None)."""
     if dz.is_cuda:
@@ -339,7 +340,8 @@ def grouped_wgrad(dz: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, rows
         _i32(rows, S, "rows")
     else:
         _check(x.shape[0] == S, f"x has {x.shape[0]} rows, dz {S}")
-    _count(max(S, x.shape[0]), "grouped_wgrad")
+    _check(S <= 0x7FFFFFFF - 255, "grouped_wgrad: more than 2^31 - 256 rows")
+    _count(x.shape[0], "grouped_wgrad")
     _check(bias or db is None, "a bias gradient buffer was given with bias=False")
     if dw is not None:
         _rows2(dw, 3, "dw")

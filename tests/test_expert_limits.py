@@ -180,3 +180,17 @@ def test_ids_of_a_weight_gradient_stay_within_32_bits(S, gathered, whole):
     for op in ("linear", "wgrad"):
         assert C.grouped_whole_words(op, 64, (1 << 28) - 32, 2, 8, 8, True)
         assert not C.grouped_whole_words(op, 64, 1 << 28, 2, 8, 8, True)
+
+
+@pytest.mark.parametrize("side", ["host", "native"])
+def test_weight_gradients_leave_room_for_a_step(side):
+    """A group's rows are counted in steps of 64, two ahead, in 32-bit integers."""
+    def call(S):
+        dz, x = torch.zeros(1, 4, dtype=BF).expand(S, 4), torch.zeros(1, 8, dtype=BF).expand(S, 8)
+        return _call(side, "grouped_wgrad", dz=dz, x=x, offsets=OFF)
+
+    with pytest.raises(RuntimeError, match="more than 2\\^31 - 256 rows"):
+        call((1 << 31) - 255)
+    if side == "native":
+        with pytest.raises(RuntimeError, match="GPU tensors"):  # only the device is wrong
+            call((1 << 31) - 256)
