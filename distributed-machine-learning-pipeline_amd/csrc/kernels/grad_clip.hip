@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const doub
   constexpr int P = gn_per<DT>();
   const double nrm = sqrt(gn_total(part, parts, lds));
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)nrm;
-  double cd = max_norm / (nrm + eps);
+  double cd = nrm + eps == 0.0 ? 1.0 : max_norm / (nrm + eps);  // nothing but zeros: not 0 / 0
   cd = cd > 1.0 ? 1.0 : cd;  // NaN stays NaN: a broken gradient is not hidden
   const float c = (float)cd;
   const uint32_t pieces = t.start[t.count];

@@ -178,7 +178,8 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float =
     _check_grads(grads, out)
     _check_written_once(grads, grads if out is None else out)
     norm = _norm_ref(grads)
-    coef = torch.clamp(max_norm / (norm + eps), max=1.0).float()
+    coef = torch.clamp(max_norm / (norm + eps), max=1.0)
+    coef = torch.where(norm + eps == 0, torch.ones_like(coef), coef).float()  # nothing but zeros: not 0 / 0
     for g, o in zip(grads, grads if out is None else out):
         o.copy_(g.float() * coef)
     return norm.float()

@@ -46,3 +46,19 @@ def test_host_takes_ranges_that_lie_apart(case):
     for (a, b), g in zip(grads if out is None else out, want):
         # the roundings of the norm, the factor and the product
         assert ((buf[a:b] - g / (n + 1e-6)).abs() <= g / n * 2.0 ** -22).all()
+
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_zero_gradients_stay_zero_whatever_the_limit(dt, dev):
+    for max_norm, eps in ((0.0, 0.0), (0.0, 1e-6), (1.0, 0.0), (float("inf"), 0.0)):
+        grads = [torch.zeros(n, dtype=dt, device=dev) for n in (3, 0, 4097)]
+        out = [torch.full_like(g, 7.0) for g in grads]
+        assert float(F.clip_grad_norm_(grads, max_norm, eps, out=out)) == 0.0
+        assert float(F.clip_grad_norm_(grads, max_norm, eps)) == 0.0
+        assert all((t == 0).all() for t in grads + out)
+    broken = [torch.zeros(5, dtype=dt, device=dev), torch.full((2,), float("nan"), dtype=dt, device=dev)]
+    assert F.clip_grad_norm_(broken, 0.0, 0.0).isnan() and all(g.isnan().all() for g in broken)
