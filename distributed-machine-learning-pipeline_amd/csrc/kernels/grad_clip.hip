@@ -164,41 +164,54 @@ __global__ __launch_bounds__(kGnThreads) void grad_norm_k(const double* part, in
   if (threadIdx.x == 0) norm[0] = (float)sqrt(s);
 }
 
-// Every workgroup sums the partials in the same order, so all scale by the same value.
-template <int DT>
-__global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const double* part, int parts, float* norm,
-                                                           double max_norm, double eps) {
-  __shared__ double lds[kGnThreads / 64];
+// g * factor over this workgroup's pieces: one fp32 product, or (FINE) one in fp64,
+// where fp32 would not hold the factor's bits.
+template <int DT, bool FINE>
+__device__ __forceinline__ void gn_scale(const GnTable& t, double factor) {
   constexpr int P = gn_per<DT>();
-  const double nrm = sqrt(gn_total(part, parts, lds));
-  if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)nrm;
-  double cd = nrm + eps == 0.0 ? 1.0 : max_norm / (nrm + eps);  // nothing but zeros: not 0 / 0
-  cd = cd > 1.0 ? 1.0 : cd;  // NaN stays NaN: a broken gradient is not hidden
-  const float c = (float)cd;
+  const float c = (float)factor;
+  auto scaled = [&](float g) { return FINE ? (float)((double)g * factor) : g * c; };
   const uint32_t pieces = t.start[t.count];
   for (uint32_t p = blockIdx.x; p < pieces; p += gridDim.x) {
     const int i = gn_find(t, p);
     const void* g = t.g[i];
     void* o = t.out[i];
-    if (c == 1.f && o == g) continue;  // nothing changes
+    if (!FINE && c == 1.f && o == g) continue;  // nothing changes
     const int64_t n = t.n[i], first = (int64_t)(p - t.start[i]) * t.piece * P;
     const int64_t last = first + (int64_t)t.piece * P < n ? first + (int64_t)t.piece * P : n;
     if (((reinterpret_cast<uintptr_t>(g) | reinterpret_cast<uintptr_t>(o)) & 15) == 0) {
       const uint4* v = reinterpret_cast<const uint4*>(g);
       uint4* w = reinterpret_cast<uint4*>(o);
       const int64_t v1 = last / P;
-      gn_words<8>(first / P, v1, [&](int64_t k) { return v[k]; }, [&](int64_t k, uint4 u) {
+      gn_words<FINE ? 1 : 8>(first / P, v1, [&](int64_t k) { return v[k]; }, [&](int64_t k, uint4 u) {
         float f[P];
         gn_unpack<DT>(u, f);
 #pragma unroll
-        for (int j = 0; j < P; ++j) f[j] *= c;
+        for (int j = 0; j < P; ++j) f[j] = scaled(f[j]);
         w[k] = gn_pack<DT>(f);
       });
-      for (int64_t k = v1 * P + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, gn_ld<DT>(g, k) * c);
+      for (int64_t k = v1 * P + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, scaled(gn_ld<DT>(g, k)));
     } else {
-      for (int64_t k = first + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, gn_ld<DT>(g, k) * c);
+      for (int64_t k = first + threadIdx.x; k < last; k += kGnThreads) gn_st<DT>(o, k, scaled(gn_ld<DT>(g, k)));
     }
   }
+}
+
+// Every workgroup sums the partials in the same order, so all scale by the same value.
+template <int DT>
+__global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const double* part, int parts, float* norm,
+                                                           double max_norm, double eps) {
+  __shared__ double lds[kGnThreads / 64];
+  const double nrm = sqrt(gn_total(part, parts, lds));
+  if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)nrm;
+  double cd = nrm + eps == 0.0 ? 1.0 : max_norm / (nrm + eps);  // nothing but zeros: not 0 / 0
+  cd = cd > 1.0 ? 1.0 : cd;  // NaN stays NaN: a broken gradient is not hidden
+  // below 2^-126 (a norm past 1e38 times the limit) fp32 drops bits of the factor;
+  // fp16 results are zeros by then
+  if constexpr (DT != kF16) {
+    if (cd > 0.0 && cd < 0x1p-126) return gn_scale<DT, true>(t, cd);
+  }
+  gn_scale<DT, false>(t, cd);
 }
 
 int64_t gn_pieces(int64_t n, int P, int piece) {

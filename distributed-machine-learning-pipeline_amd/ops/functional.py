@@ -179,7 +179,9 @@ def clip_grad_norm_(grads: Sequence[torch.Tensor], max_norm: float, eps: float =
     _check_written_once(grads, grads if out is None else out)
     norm = _norm_ref(grads)
     coef = torch.clamp(max_norm / (norm + eps), max=1.0)
-    coef = torch.where(norm + eps == 0, torch.ones_like(coef), coef).float()  # nothing but zeros: not 0 / 0
+    coef = torch.where(norm + eps == 0, torch.ones_like(coef), coef)  # nothing but zeros: not 0 / 0
+    # below 2^-126 float32 drops bits of the factor: a product in float64 there
+    fine = 0.0 < float(coef) < 2.0 ** -126
     for g, o in zip(grads, grads if out is None else out):
-        o.copy_(g.float() * coef)
+        o.copy_((g.double() * coef).float() if fine else g.float() * coef.float())
     return norm.float()

@@ -62,3 +62,23 @@ def test_zero_gradients_stay_zero_whatever_the_limit(dt, dev):
         assert all((t == 0).all() for t in grads + out)
     broken = [torch.zeros(5, dtype=dt, device=dev), torch.full((2,), float("nan"), dtype=dt, device=dev)]
     assert F.clip_grad_norm_(broken, 0.0, 0.0).isnan() and all(g.isnan().all() for g in broken)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("max_norm", [3.0, 1e-3, 1e-30])
+def test_a_factor_below_float32s_normal_range_keeps_its_bits(max_norm, dt, dev):
+    """Gradients near the type's largest value: the factor is below 2^-126, the clipped
+    values are not."""
+    g = torch.linspace(0.5, 1.0, 4099, dtype=torch.float64)
+    grads = [(s * g * 3e38).to(dt).to(dev) for s in (1.0, -0.5)]
+    out = [torch.empty_like(t) for t in grads]
+    n = sum(t.double().square().sum() for t in grads).sqrt()
+    want = [t.double() * (max_norm / n) for t in grads]
+    assert max_norm / float(n) < 2.0 ** -126
+    F.clip_grad_norm_(grads, max_norm, 0.0, out=out)
+    F.clip_grad_norm_(grads, max_norm, 0.0)
+    for a, o, w in zip(grads, out, want):
+        assert torch.equal(a, o)
+        # the product's rounding and the type's
+        assert ((a.double() - w).abs() <= w.abs() * (2.0 ** -23 + torch.finfo(dt).eps / 2)).all()
