@@ -17,6 +17,7 @@
 // (5.5 TB/s) and 600 for the scaling (5.3 TB/s, read and write).  109386 in 6: 7.7 us
 // in the two kernels; the host needs 10 to call.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "../dsml.h"
@@ -213,6 +214,16 @@ __global__ __launch_bounds__(kGnThreads) void grad_scale_k(GnTable t, const doub
   }
   gn_scale<DT, false>(t, cd);
 }
+
+// gn_find reads the table where the first argument lies.
+template <class F>
+struct GnFirst;
+template <class A, class... R>
+struct GnFirst<void (*)(A, R...)> {
+  using type = A;
+};
+static_assert(std::is_same_v<GnFirst<decltype(&grad_sq_k<kF32>)>::type, GnTable>, "the table comes first");
+static_assert(std::is_same_v<GnFirst<decltype(&grad_scale_k<kF32>)>::type, GnTable>, "the table comes first");
 
 int64_t gn_pieces(int64_t n, int P, int piece) {
   const int64_t per = (int64_t)piece * P;
