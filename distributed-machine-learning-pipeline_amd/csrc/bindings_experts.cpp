@@ -453,7 +453,7 @@ torch::Tensor py_grad_norm(const std::vector<torch::Tensor>& grads, bool clip, d
   }
   TORCH_CHECK(gpu, "gradients must be on one GPU");
   OnDevice on(grads[0]);
-  const int64_t words = grad_norm_ws_doubles(nullptr, (int)t.size());
+  const int64_t words = grad_norm_ws_doubles((int)t.size());
   torch::Tensor ws = torch::empty({words}, grads[0].options().dtype(torch::kFloat64));
   torch::Tensor norm = torch::empty({}, grads[0].options().dtype(torch::kFloat32));
   ex_hip_ok(grad_norm(t.data(), (int)t.size(), dt, ws.data_ptr<double>(), norm.data_ptr<float>(), clip, max_norm, eps,

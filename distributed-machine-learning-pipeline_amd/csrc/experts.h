@@ -110,8 +110,8 @@ struct ClipTensor {
   void* out;  // == g: in place
   int64_t n;
 };
-// Floats of workspace: doubles hold the partial sums (grad_norm_ws_doubles).
-int64_t grad_norm_ws_doubles(const int64_t* n, int count);
+// Doubles of workspace: the partial sums of `count` tensors.
+int64_t grad_norm_ws_doubles(int count);
 // norm[0] = sqrt(sum g^2); clip: out = g * min(1, max_norm / (norm + eps)).
 hipError_t grad_norm(const ClipTensor* t, int count, int dtype, double* ws, float* norm, bool clip, double max_norm,
                      double eps, hipStream_t s);

@@ -8,10 +8,12 @@
 // waits for bytes, not for arithmetic).  Two passes: the first leaves one fp64
 // partial per workgroup, every workgroup of the second sums all of them in
 // the same order -- no atomics, so the result does not depend on timing -- and
-// scales its share.  Tensors are cut into pieces of 256 to 4096 16-B words (about
-// 1024 pieces in all, each thread's words of one requested together); a workgroup
-// takes every gridDim-th piece.  The tensor table travels in the kernel
-// arguments, so a call keeps nothing on the device and can be captured.
+// scales its share.  Tensors are cut into pieces of 256 to 4096 16-B words: about
+// 1024 pieces in all while 4096 words are enough for that (400 M fp32 gradients are
+// 24415 of them), of which a workgroup takes every gridDim-th, 8 words a thread in
+// flight.  The tensor table travels in the kernel arguments, so a call keeps
+// nothing on the device and can be captured.  Tensors that do not start at a
+// multiple of 16 B go element by element.
 //
 // 400 M fp32 gradients in 60 tensors, clipped into others: 899 us, 290 for the norm
 // (5.5 TB/s) and 600 for the scaling (5.3 TB/s, read and write).  109386 in 6: 7.7 us
@@ -243,9 +245,8 @@ int gn_grid(int64_t pieces, int64_t all) {
 
 }  // namespace
 
-int64_t grad_norm_ws_doubles(const int64_t* n, int count) {
+int64_t grad_norm_ws_doubles(int count) {
   // every launch rounds its share up by at most one workgroup
-  (void)n;
   return kGnBlocks + (count + kGnMax - 1) / kGnMax + 1;
 }
 

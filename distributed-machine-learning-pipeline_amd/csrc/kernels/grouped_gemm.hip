@@ -187,9 +187,11 @@ __device__ __forceinline__ GgTile gg_find(const int32_t* off, int E, int64_t S, 
 //
 // bf16, 8 experts: 32768 rows x 4096 x 4096 851 us (1292 TFLOP/s; 1535 for a plain
 // library product of that size), the input gradient of 16384 rows 493 (1115), the
-// weight gradient 493 (1116).  With random data the matrix units run at the power
-// limit (788 us of a step count alike on zeros); outside of the products a tile
-// costs about 8 us: its stores, its search, its first loads.
+// weight gradient 493 (1116); up to 4 % more on some cards.  With random data the
+// first runs at the power limit (1.73 GHz, matrix units 64 % busy; 788 us of a step
+// count alike on zeros), the gradients do not (2.04 and 2.09 GHz, 56 and 47 %);
+// outside of the products a tile costs about 8 us: its stores, its search, its
+// first loads.
 // ---------------------------------------------------------------------------
 typedef __attribute__((address_space(3))) void* gg_lptr;
 typedef short gg_i16x4 __attribute__((ext_vector_type(4)));
@@ -871,7 +873,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void grouped_fast_k(GroupedArgs a,
 // the time.  A workgroup owns 64 output columns of up to 16 MX rows; its 4 waves
 // take the 64-deep steps in turn, each with a ring of its own (2 slots of 64
 // weight rows and 16 MX operand rows), so the loop has no barrier and 4 x 2 slots
-// a workgroup, two workgroups a CU, are in flight.  The waves' partial tiles are
+// a workgroup are in flight, of two workgroups a CU (MX 1: 80 KiB of LDS) or one
+// (MX 2: 96 KiB).  The waves' partial tiles are
 // summed in wave order through LDS.  16 rows, 8 experts of 4096 x 4096: 54 us with
 // cold weights (4.9 TB/s), 92 with 128 x 128 tiles.
 // ---------------------------------------------------------------------------
@@ -1052,7 +1055,10 @@ __global__ __launch_bounds__(256, 2) void grouped_skinny_k(GroupedArgs a, int nt
 // operands that the fast path takes too it needs 51 us against 37 (8192 rows, 8
 // experts of 1000 x 1000) and 1415 against 980 (32768 of 4096 x 4096); 8192 rows of
 // 1003 x 1001 with a bias: 36 (44 with the bias loaded at its use; backward with a
-// mask 46 and 52).
+// mask 46 and 52).  Against the same sizes rounded up to whole words: 5003 rows, 4
+// experts of 301 x 2003, 29 us against 18; 2000 rows of 1001 x 1003 27 and 14; 16 rows,
+// 8 experts of 4001 x 4095, 92 and 49; the weight gradient of 8192 rows of 127 x 783
+// 23 and 16.
 // ---------------------------------------------------------------------------
 // Loads are never under a condition (the compiler waits for such a load at the
 // end of its branch: 115 us against 58 at 8192 rows, 8 experts of 1003 x 1001):
@@ -1577,7 +1583,8 @@ hipError_t launch_fast_op(GroupedOp op, const GroupedArgs& a, hipStream_t s) {
   // 128 x 128 tiles are fewer than the CUs, each of them a long chain of steps (8
   // experts of 1024 x 4096, microseconds, 128 x 128 after the slash: 32 rows an
   // expert 16 / 36, 96 29 / 38, 128 40 / 39; of 1024 x 1024: 32 6 / 12, 96 11 / 13,
-  // 128 15 / 14), that is while its workgroups fit the chip about once, two a CU.
+  // 128 15 / 14).  32 rows a tile leave one workgroup a CU: the limits, two rounds of
+  // the chip and two and a half, lie between those sizes.
   // With 16 rows a tile while experts have no more (4096 x 4096: 8 rows 44 / 52, 16
   // 46 / 55; backward 45 / 42 and 52 / 47), else 32 (24 rows: 47 against 50, and 55).
   const int red = op == kLinear ? a.K : a.N, cols = op == kLinear ? a.N : a.K;
