@@ -10,7 +10,7 @@
 // the same order -- no atomics, so the result does not depend on timing -- and
 // scales its share.  Tensors are cut into pieces of 256 to 4096 16-B words: about
 // 1024 pieces in all while 4096 words are enough for that (400 M fp32 gradients are
-// 24415 of them), of which a workgroup takes every gridDim-th, 8 words a thread in
+// some 24400 of them), of which a workgroup takes every gridDim-th, 8 words a thread in
 // flight.  The tensor table travels in the kernel arguments, so a call keeps
 // nothing on the device and can be captured.  Tensors that do not start at a
 // multiple of 16 B go element by element.
